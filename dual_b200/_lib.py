@@ -65,6 +65,15 @@ SIGNATURES = {
         VP, VP, C.c_int64, C.c_int64, VP, VP, VP, VP, VP, C.c_int, C.c_int, C.c_int, VP, C.c_int, VP]),
     "dual_set_kv_buffer": (C.c_int, [
         VP, VP, C.c_int64, C.c_int64, VP, C.c_int64, VP, C.c_int64, VP, C.c_int, C.c_int64, VP, C.c_int, VP]),
+    "dual_rope_set_kv_buffer": (C.c_int, [
+        VP, VP, C.c_int64, C.c_int64,          # k_local, v_local, local stride, capacity
+        VP, C.c_int, VP, C.c_int,              # locations, is int64, positions, is int64
+        VP, C.c_int64, C.c_int, C.c_int,       # cos_sin, max positions, rotary dim, interleaved
+        VP, C.c_int64, VP, C.c_int64, VP, C.c_int64, VP, C.c_int64,  # q, k, v, q_out with token strides
+        VP, VP, C.c_double, C.c_int64, VP, C.c_int, VP]),  # norm weights, eps, n, status, device, stream
+    "dual_merge_attention_states": (C.c_int, [
+        VP, VP, VP, VP, C.c_int, C.c_int, C.c_int64,  # states, strides, lses, count, fp32, tokens
+        VP, C.c_int64, C.c_int64, C.c_int, VP, C.c_int, VP]),  # out, strides, fp32, lse, device, stream
     "dual_migrate_copy": (C.c_int, [
         VP, VP, C.c_int, C.c_int, VP, VP, C.c_int64, C.c_int, C.c_int64, C.c_int64, C.c_int64, VP, C.c_int,
         C.c_int, VP]),
@@ -95,6 +104,7 @@ STATUS_BITS = {
     0x8: "bad copy slot",
     0x10: "bad length",
     0x20: "bad tier value",
+    0x40: "bad position",
 }
 
 

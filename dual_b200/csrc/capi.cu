@@ -10,9 +10,11 @@
 #include "decode.cuh"
 #include "device_guard.h"
 #include "kv_write.cuh"
+#include "merge.cuh"
 #include "migrate.cuh"
 #include "pack.cuh"
 #include "prefill.cuh"
+#include "rope_kv.cuh"
 #include "stage.cuh"
 
 namespace {
@@ -435,6 +437,104 @@ int dual_set_kv_buffer(void* k_local, void* v_local, int64_t local_stride_bytes,
   p.status = status;
   cudaError_t e = dual::launch_set_kv_buffer(p, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "set_kv_buffer launch");
+  return DUAL_OK;
+}
+
+int dual_rope_set_kv_buffer(void* k_local, void* v_local, int64_t local_stride_bytes, int64_t local_capacity,
+                            const void* locations, int loc_is_int64, const void* positions, int pos_is_int64,
+                            const float* cos_sin, int64_t max_positions, int rotary_dim, int interleaved,
+                            const void* q, int64_t q_stride_token, const void* k, int64_t k_stride_token,
+                            const void* v, int64_t v_stride_token, void* q_out, int64_t q_out_stride_token,
+                            const void* q_norm_weight, const void* k_norm_weight, double norm_eps, int64_t n,
+                            uint32_t* status, int device, void* stream) {
+  g_last_error.clear();
+  if (n < 0) return fail(DUAL_EINVAL, "n must be >= 0");
+  if (n == 0) return DUAL_OK;
+  if (!k_local || !v_local || !locations || !positions || !cos_sin || !q || !k || !v || !q_out || !status)
+    return fail(DUAL_EINVAL, "null pointer argument");
+  const int64_t row = int64_t(dual::kNumKvHeads) * dual::kHeadDim, q_row = int64_t(dual::kNumQoHeads) * dual::kHeadDim;
+  if (!aligned16(k_local) || !aligned16(v_local) || (local_stride_bytes & 15) || local_stride_bytes < row * 2)
+    return fail(DUAL_EINVAL, "local pools must be 16-byte aligned with a slot stride >= 2048 B, multiple of 16");
+  if (local_capacity < 0) return fail(DUAL_EINVAL, "local_capacity must be >= 0");
+  if (rotary_dim < 16 || rotary_dim > dual::kHeadDim || rotary_dim % 16)
+    return fail(DUAL_EINVAL, "rotary_dim must be a multiple of 16 in [16, %d] (got %d)", dual::kHeadDim, rotary_dim);
+  if (max_positions <= 0 || !aligned16(cos_sin))
+    return fail(DUAL_EINVAL, "cos_sin must be 16-byte aligned with at least one position");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) || (q_stride_token % 8) ||
+      (k_stride_token % 8) || (v_stride_token % 8) || (q_out_stride_token % 8) || q_stride_token < q_row ||
+      q_out_stride_token < q_row || k_stride_token < row || v_stride_token < row)
+    return fail(DUAL_EINVAL, "q/q_out/k/v must be 16-byte aligned with token strides that are multiples of 8 elements "
+                             "and hold a token's heads (4096 or 1024 elements)");
+  if (!aligned16(q_norm_weight) || !aligned16(k_norm_weight))
+    return fail(DUAL_EINVAL, "norm weights must be 16-byte aligned");
+  if (!(norm_eps >= 0.0)) return fail(DUAL_EINVAL, "norm_eps must be >= 0");
+  DUAL_USE_DEVICE(device);
+  dual::RopeKvParams p{};
+  p.k_local = static_cast<char*>(k_local);
+  p.v_local = static_cast<char*>(v_local);
+  p.local_stride = local_stride_bytes;
+  p.capacity = local_capacity;
+  p.loc = locations;
+  p.loc64 = loc_is_int64;
+  p.pos = positions;
+  p.pos64 = pos_is_int64;
+  p.cos_sin = cos_sin;
+  p.max_pos = max_positions;
+  p.rotary = rotary_dim;
+  p.interleaved = interleaved ? 1 : 0;
+  p.q = static_cast<const char*>(q);
+  p.k = static_cast<const char*>(k);
+  p.v = static_cast<const char*>(v);
+  p.q_stride = q_stride_token * 2;
+  p.k_stride = k_stride_token * 2;
+  p.v_stride = v_stride_token * 2;
+  p.q_out = static_cast<char*>(q_out);
+  p.q_out_stride = q_out_stride_token * 2;
+  p.q_norm = static_cast<const __nv_bfloat16*>(q_norm_weight);
+  p.k_norm = static_cast<const __nv_bfloat16*>(k_norm_weight);
+  p.eps = static_cast<float>(norm_eps);
+  p.n = n;
+  p.status = status;
+  cudaError_t e = dual::launch_rope_set_kv_buffer(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "rope_set_kv_buffer launch");
+  return DUAL_OK;
+}
+
+int dual_merge_attention_states(const void* const* states, const int64_t* stride_token, const int64_t* stride_head,
+                                const float* const* state_lse, int num_states, int states_fp32, int64_t tokens,
+                                void* out, int64_t out_stride_token, int64_t out_stride_head, int out_fp32, float* lse,
+                                int device, void* stream) {
+  g_last_error.clear();
+  if (tokens < 0) return fail(DUAL_EINVAL, "tokens must be >= 0");
+  if (num_states < 1 || num_states > dual::kMaxStates)
+    return fail(DUAL_EINVAL, "num_states must be in [1, %d] (got %d)", dual::kMaxStates, num_states);
+  if (tokens == 0) return DUAL_OK;
+  if (tokens > (int64_t(1) << 27)) return fail(DUAL_EINVAL, "too many tokens");
+  if (!states || !stride_token || !stride_head || !state_lse || !out) return fail(DUAL_EINVAL, "null pointer argument");
+  const int in_step = states_fp32 ? 4 : 8, out_step = out_fp32 ? 4 : 8;
+  for (int i = 0; i < num_states; ++i) {
+    if (!states[i] || !state_lse[i]) return fail(DUAL_EINVAL, "state %d: null pointer", i);
+    if (!aligned16(states[i]) || (stride_token[i] % in_step) || (stride_head[i] % in_step))
+      return fail(DUAL_EINVAL, "state %d must be 16-byte aligned with strides that are multiples of 16 bytes", i);
+  }
+  if (!aligned16(out) || (out_stride_token % out_step) || (out_stride_head % out_step))
+    return fail(DUAL_EINVAL, "out must be 16-byte aligned with strides that are multiples of 16 bytes");
+  DUAL_USE_DEVICE(device);
+  dual::MergeParams p{};
+  for (int i = 0; i < num_states; ++i) {
+    p.o[i] = states[i];
+    p.stride_tok[i] = stride_token[i];
+    p.stride_head[i] = stride_head[i];
+    p.lse[i] = state_lse[i];
+  }
+  p.states = num_states;
+  p.tokens = tokens;
+  p.out = out;
+  p.out_stride_tok = out_stride_token;
+  p.out_stride_head = out_stride_head;
+  p.lse_out = lse;
+  cudaError_t e = dual::launch_merge_states(p, states_fp32 != 0, out_fp32 != 0, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "merge_attention_states launch");
   return DUAL_OK;
 }
 

@@ -40,6 +40,7 @@ enum StatusBits : unsigned {
   kStatusWaitTimeout = 1u << 2,    // a bounded mbarrier wait gave up
   kStatusBadCopySlot = 1u << 3,    // migration source/target outside its pool
   kStatusBadLength = 1u << 4,      // negative length / indptr not monotone
+  kStatusBadPosition = 1u << 6,    // position outside the rotation table
 };
 
 // Wall-clock bound on any spin-wait in our kernels: ~1 s, then the kernel

@@ -224,6 +224,107 @@ def set_kv_buffer(k_local: torch.Tensor, v_local: torch.Tensor, locations: torch
         _stream(k_local.device)))
 
 
+def _on_device(device: torch.device, **tensors: Optional[torch.Tensor]) -> None:
+    for name, t in tensors.items():
+        _check(t is None or t.device == device, f"{name} must be on {device}")
+
+
+def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two views [n, heads, dims] share memory: rows at one token stride that lie side by side in
+    one buffer (a fused projection's q | k | v) do not, the same view does."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    size = lambda t: t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))  # noqa: E731
+    lo, hi = sorted((a, b), key=lambda t: t.data_ptr())
+    if lo.data_ptr() + size(lo) <= hi.data_ptr():
+        return False
+    step = a.stride(0) * a.element_size()
+    if step and step == b.stride(0) * b.element_size():
+        at = (hi.data_ptr() - lo.data_ptr()) % step
+        return not (size(lo[:1]) <= at and at + size(hi[:1]) <= step)
+    return True
+
+
+def _same_view(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return (a.data_ptr(), a.dtype, a.shape, a.stride()) == (b.data_ptr(), b.dtype, b.shape, b.stride())
+
+
+def rope_set_kv_buffer(k_local: torch.Tensor, v_local: torch.Tensor, locations: torch.Tensor,
+                       positions: torch.Tensor, cos_sin: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                       v: torch.Tensor, q_out: torch.Tensor, status: torch.Tensor, *, interleaved: bool = False,
+                       q_norm_weight: Optional[torch.Tensor] = None, k_norm_weight: Optional[torch.Tensor] = None,
+                       norm_eps: float = 1e-6) -> None:
+    """``set_kv_buffer`` with the position rotation on the way: ``q`` [n, 32, 128] rotated into ``q_out``
+    (which may be ``q``), ``k`` [n, 8, 128] rotated and ``v`` as it is into local slots ``locations`` of one
+    layer's pools.  ``positions`` [n] name rows of ``cos_sin`` (fp32 [positions, rotary dims]: cosines, then
+    sines); the first ``rotary dims`` of each head are turned, in pairs (j, j + half) or, ``interleaved``,
+    (2j, 2j + 1).  With norm weights [128] bf16 each q / k head row is RMS-normalised first.  Token strides
+    are free (views of a fused qkv buffer).  Tokens with a bad position are skipped, rows with a bad slot are
+    not stored; both are recorded in ``status``."""
+    ls = _pool_stride(k_local, "k_local")
+    _check(_pool_stride(v_local, "v_local") == ls and v_local.shape[0] == k_local.shape[0],
+           "k/v local pools must share a slot stride and a size")
+    n = locations.numel()
+    for t, heads, name in ((q, NUM_QO_HEADS, "q"), (q_out, NUM_QO_HEADS, "q_out"), (k, NUM_KV_HEADS, "k"),
+                           (v, NUM_KV_HEADS, "v")):
+        _check(t.dtype == torch.bfloat16 and t.dim() == 3 and tuple(t.shape) == (n, heads, HEAD_DIM)
+               and (n == 0 or (t.stride(2) == 1 and t.stride(1) == HEAD_DIM)),
+               f"{name} must be bf16 [n, {heads}, 128] with heads x dims contiguous")
+    for t, name in ((locations, "locations"), (positions, "positions")):
+        _check(t.dtype in (torch.int64, torch.int32) and t.dim() == 1 and t.numel() == n and t.is_contiguous(),
+               f"{name} must be contiguous int64/int32 [n]")
+    _check(cos_sin.dtype == torch.float32 and cos_sin.dim() == 2 and cos_sin.is_contiguous(),
+           "cos_sin must be contiguous fp32 [positions, rotary dims]")
+    for t, name in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
+        _check(t is None or (t.dtype == torch.bfloat16 and tuple(t.shape) == (HEAD_DIM,) and t.is_contiguous()),
+               f"{name} must be contiguous bf16 [128]")
+    _check(status.dtype in (torch.int32, torch.uint32) and status.numel() >= 1, "status must be a 32-bit word")
+    _on_device(k_local.device, v_local=v_local, locations=locations, positions=positions, cos_sin=cos_sin, q=q, k=k,
+               v=v, q_out=q_out, status=status, q_norm_weight=q_norm_weight, k_norm_weight=k_norm_weight)
+    _check(_same_view(q_out, q) or not _overlaps(q_out, q), "q_out must be q itself or not overlap it")
+    _check(not _overlaps(q_out, k) and not _overlaps(q_out, v), "q_out must not overlap k or v")
+    # one token has no stride of its own
+    st = lambda t, heads: t.stride(0) if n > 1 else heads * HEAD_DIM  # noqa: E731
+    lib = _lib.load()
+    _lib.check(lib.dual_rope_set_kv_buffer(
+        k_local.data_ptr(), v_local.data_ptr(), ls, k_local.shape[0] - 1, locations.data_ptr(),
+        int(locations.dtype == torch.int64), positions.data_ptr(), int(positions.dtype == torch.int64),
+        cos_sin.data_ptr(), cos_sin.shape[0], cos_sin.shape[1], int(bool(interleaved)), q.data_ptr(),
+        st(q, NUM_QO_HEADS), k.data_ptr(), st(k, NUM_KV_HEADS), v.data_ptr(), st(v, NUM_KV_HEADS), q_out.data_ptr(),
+        st(q_out, NUM_QO_HEADS), _ptr(q_norm_weight), _ptr(k_norm_weight), float(norm_eps), n, status.data_ptr(),
+        _dev(k_local), _stream(k_local.device)))
+
+
+def merge_attention_states(states: Sequence[torch.Tensor], lses: Sequence[torch.Tensor], out: torch.Tensor,
+                           lse: Optional[torch.Tensor] = None) -> None:
+    """Join 1 to 8 partial attention states of the same queries over disjoint keys (what
+    ``run_return_lse`` returns): ``states[i]`` [T, 32, 128], all bf16 or all fp32, ``lses[i]`` fp32 [T, 32]
+    (base 2).  ``out`` [T, 32, 128] bf16 or fp32 and ``lse`` [T, 32] (optional) may be one of them."""
+    n = len(states)
+    _check(1 <= n <= 8 and len(lses) == n, "need 1 to 8 states, each with its lse")
+    T = out.shape[0]
+    for t, name in [(out, "out")] + [(s, f"states[{i}]") for i, s in enumerate(states)]:
+        _check(t.dtype in (torch.bfloat16, torch.float32) and tuple(t.shape) == (T, NUM_QO_HEADS, HEAD_DIM)
+               and (T == 0 or t.stride(2) == 1), f"{name} must be bf16 or fp32 [T, 32, 128] with contiguous head_dim")
+    _check(all(s.dtype == states[0].dtype for s in states), "states must share a type")
+    for t, name in [(lse, "lse")] + [(l, f"lses[{i}]") for i, l in enumerate(lses)]:
+        _check(t is None and name == "lse" or (t.dtype == torch.float32 and tuple(t.shape) == (T, NUM_QO_HEADS)
+                                               and t.is_contiguous()), f"{name} must be contiguous fp32 [T, 32]")
+    _on_device(out.device, lse=lse, **{f"states[{i}]": s for i, s in enumerate(states)},
+               **{f"lses[{i}]": l for i, l in enumerate(lses)})
+    for s in states:
+        _check(_same_view(out, s) or not _overlaps(out, s), "out must be one of the states or not overlap them")
+    for t in lses if lse is not None else ():
+        _check(_same_view(lse, t) or not _overlaps(lse, t), "lse must be one of the lses or not overlap them")
+    arr = lambda vs: (C.c_int64 * n)(*vs)  # noqa: E731
+    st = lambda t: t.stride(0) if T > 1 else NUM_QO_HEADS * HEAD_DIM  # noqa: E731
+    lib = _lib.load()
+    _lib.check(lib.dual_merge_attention_states(
+        _ptrs(states), arr([st(s) for s in states]), arr([s.stride(1) for s in states]), _ptrs(lses), n,
+        int(states[0].dtype == torch.float32), T, out.data_ptr(), st(out), out.stride(1),
+        int(out.dtype == torch.float32), _ptr(lse), _dev(out), _stream(out.device)))
+
+
 def migrate_copy(local_planes: torch.Tensor, remote_planes: torch.Tensor, num_planes: int, num_banks: int,
                  source: torch.Tensor, target: torch.Tensor, reverse: bool, local_slots: int,
                  remote_slots: int, status: torch.Tensor, row_bytes: int = SLOT_BYTES, max_ctas: int = 0) -> None:

@@ -36,6 +36,7 @@ extern "C" {
 #define DUAL_STATUS_BAD_COPY_SLOT 0x8u
 #define DUAL_STATUS_BAD_LENGTH 0x10u
 #define DUAL_STATUS_BAD_TIER 0x20u
+#define DUAL_STATUS_BAD_POSITION 0x40u
 
 /* Thread-local message of the last failing call ("" if none). */
 const char* dual_last_error(void);
@@ -194,6 +195,46 @@ int dual_set_kv_buffer(void* k_local, void* v_local, int64_t local_stride_bytes,
                        const void* k, int64_t k_stride_token, const void* v, int64_t v_stride_token,
                        const void* locations, int loc_is_int64, int64_t n, uint32_t* status, int device,
                        void* stream);
+
+/* The KV writer with the position rotation applied on the way (no counterpart in the reference, whose
+ * model rotates q and k in kernels of their own before set_kv_buffer).  For token i < n with position
+ * p = positions[i] and slot s = locations[i]:
+ *   q_out[i] = R_p(q[i]);   k_local[s] = R_p(k[i]);   v_local[s] = v[i] (bit-exact).
+ * R_p rotates the first rotary_dim (a multiple of 16, 16..128) of each head's 128 dims: with
+ * c_j = cos_sin[p][j], s_j = cos_sin[p][rotary_dim / 2 + j], j < rotary_dim / 2,
+ *   (a, b) -> (a c_j - b s_j, b c_j + a s_j) for (a, b) = dims (j, j + rotary_dim / 2), or dims
+ *   (2j, 2j + 1) when interleaved != 0; the other dims stay as they are.
+ * q_norm_weight / k_norm_weight (each [128] bf16, or NULL for none): the head row is first scaled to
+ * x * weight / sqrt(mean(x^2) + norm_eps) over its 128 dims.  All in 32 bits, rounded once to bf16.
+ * cos_sin: fp32 [max_positions, rotary_dim], contiguous.  q / q_out [n, 32, 128], k / v [n, 8, 128] bf16,
+ * heads x dims contiguous, token strides in elements.  q_out may be q itself; otherwise q, k, v, q_out and
+ * the pools do not overlap.  positions / locations are int64 or int32 each.
+ * A position outside [0, max_positions): nothing of the token is written, DUAL_STATUS_BAD_POSITION.
+ * A slot outside [0, local_capacity]: its K / V rows are skipped (q_out is written),
+ * DUAL_STATUS_BAD_LOCAL_SLOT.  Slots named twice in a call (padded entries that share the dummy slot 0)
+ * end up with rows of any of their tokens, in parts. */
+int dual_rope_set_kv_buffer(void* k_local, void* v_local, int64_t local_stride_bytes, int64_t local_capacity,
+                            const void* locations, int loc_is_int64, const void* positions, int pos_is_int64,
+                            const float* cos_sin, int64_t max_positions, int rotary_dim, int interleaved,
+                            const void* q, int64_t q_stride_token, const void* k, int64_t k_stride_token,
+                            const void* v, int64_t v_stride_token, void* q_out, int64_t q_out_stride_token,
+                            const void* q_norm_weight, const void* k_norm_weight, double norm_eps, int64_t n,
+                            uint32_t* status, int device, void* stream);
+
+/* Joins num_states (1..8) partial attention states of the same queries over disjoint sets of keys, as
+ * the reference's ragged cascade does for history and chunk (peer/cascade_oracle.py:21-28): with
+ * m = max_i lse_i and w_i = 2^(lse_i - m),
+ *   out = sum_i w_i state_i / sum_i w_i,   lse = m + log2 sum_i w_i.
+ * A state with weight 0 (lse -inf: no keys) counts nothing whatever its values; where every state has
+ * lse -inf, out = 0 and lse = -inf.  In 32 bits, rounded once.
+ * states: host array of device pointers to [tokens, 32, 128] bf16 (fp32 when states_fp32), strides in
+ * elements per state (host arrays), the 128 dims contiguous; state_lse: host array of device pointers to
+ * contiguous fp32 [tokens, 32], base 2.  out bf16 (fp32 when out_fp32) and lse (or NULL) may be one of
+ * the states (same type and strides) and one of the state_lse; they do not overlap them otherwise. */
+int dual_merge_attention_states(const void* const* states, const int64_t* stride_token, const int64_t* stride_head,
+                                const float* const* state_lse, int num_states, int states_fp32, int64_t tokens,
+                                void* out, int64_t out_stride_token, int64_t out_stride_head, int out_fp32, float* lse,
+                                int device, void* stream);
 
 /* ------------------------------------------------------------- migration ---
  * Replaces Triton fused_copy._copy / copy_pages / restore (peer/fused_copy.py:6-33):
