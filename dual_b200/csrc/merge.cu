@@ -51,57 +51,77 @@ __device__ __forceinline__ void store(__nv_bfloat16* dst, const float* x) {
     *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
 }
 
-template <typename In, typename Out>
+// R rows per thread and at most kMaxStates / R states: a thread has about eight loads in flight either way.
+template <typename In, typename Out, int R>
 __global__ void __launch_bounds__(kMergeThreads) merge_states_kernel(const __grid_constant__ MergeParams p) {
-  constexpr int E = Chunk<In>::kElems, kLanes = kHeadDim / E, kRows = kMergeThreads / kLanes;
+  constexpr int E = Chunk<In>::kElems, kLanes = kHeadDim / E, kRows = kMergeThreads / kLanes, kStates = kMaxStates / R;
   const int c = threadIdx.x % kLanes;
-  const int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / kLanes;
-  const bool valid = row < p.tokens * kNumQoHeads;
-  const int64_t tok = valid ? row / kNumQoHeads : 0;
-  const int head = valid ? int(row % kNumQoHeads) : 0;
-  uint4 raw[kMaxStates];
-  float l[kMaxStates];
-  float m = -INFINITY;
+  const int64_t first = int64_t(blockIdx.x) * (kRows * R) + threadIdx.x / kLanes;
+  const int64_t rows = p.tokens * kNumQoHeads;
+  uint4 raw[R][kStates];
+  float l[R][kStates];
 #pragma unroll
-  for (int s = 0; s < kMaxStates; ++s) {
-    if (s >= p.states) break;
-    raw[s] = *reinterpret_cast<const uint4*>(static_cast<const In*>(p.o[s]) + tok * p.stride_tok[s] +
-                                             head * p.stride_head[s] + c * E);
-    l[s] = p.lse[s][tok * kNumQoHeads + head];
+  for (int r = 0; r < R; ++r) {
+    const int64_t row = min(first + r * kRows, rows - 1);
+    const int64_t tok = row / kNumQoHeads;
+    const int head = int(row % kNumQoHeads);
+#pragma unroll
+    for (int s = 0; s < kStates; ++s) {
+      if (s >= p.states) break;
+      raw[r][s] = *reinterpret_cast<const uint4*>(static_cast<const In*>(p.o[s]) + tok * p.stride_tok[s] +
+                                                  head * p.stride_head[s] + c * E);
+      l[r][s] = p.lse[s][row];
+    }
   }
+  __syncthreads();  // every lane of a row has read its log-sum-exps before one of them may be overwritten
 #pragma unroll
-  for (int s = 0; s < kMaxStates; ++s) {
-    if (s >= p.states) break;
-    m = fmaxf(m, l[s]);
+  for (int r = 0; r < R; ++r) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < kStates; ++s) {
+      if (s >= p.states) break;
+      m = fmaxf(m, l[r][s]);
+    }
+    if (m == -INFINITY) m = 0.f;
+    float acc[E], total = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int s = 0; s < kStates; ++s) {
+      if (s >= p.states) break;
+      const float w = exp2f(l[r][s] - m);
+      total += w;
+      float x[E];
+      Chunk<In>::unpack(raw[r][s], x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += w > 0.f ? w * x[e] : 0.f;
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= inv;
+    const int64_t row = first + r * kRows;
+    if (row >= rows) continue;
+    store<E>(static_cast<Out*>(p.out) + (row / kNumQoHeads) * p.out_stride_tok + (row % kNumQoHeads) * p.out_stride_head +
+                 c * E, acc);
+    if (c == 0 && p.lse_out != nullptr) p.lse_out[row] = m + log2f(total);
   }
-  if (m == -INFINITY) m = 0.f;
-  float acc[E], total = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll
-  for (int s = 0; s < kMaxStates; ++s) {
-    if (s >= p.states) break;
-    const float w = exp2f(l[s] - m);
-    total += w;
-    float x[E];
-    Chunk<In>::unpack(raw[s], x);
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += w > 0.f ? w * x[e] : 0.f;
-  }
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] *= inv;
-  __syncwarp();  // every lane of a row has read its log-sum-exps before one of them may be overwritten
-  if (!valid) return;
-  store<E>(static_cast<Out*>(p.out) + tok * p.out_stride_tok + head * p.out_stride_head + c * E, acc);
-  if (c == 0 && p.lse_out != nullptr) p.lse_out[tok * kNumQoHeads + head] = m + log2f(total);
+}
+
+template <typename In, typename Out, int R>
+void launch_rows(const MergeParams& p, cudaStream_t stream) {
+  constexpr int kRows = kMergeThreads / (kHeadDim / Chunk<In>::kElems) * R;
+  const int64_t rows = p.tokens * kNumQoHeads;
+  merge_states_kernel<In, Out, R><<<unsigned((rows + kRows - 1) / kRows), kMergeThreads, 0, stream>>>(p);
 }
 
 template <typename In, typename Out>
 void launch(const MergeParams& p, cudaStream_t stream) {
-  constexpr int kRows = kMergeThreads / (kHeadDim / Chunk<In>::kElems);
-  const int64_t rows = p.tokens * kNumQoHeads;
-  merge_states_kernel<In, Out><<<unsigned((rows + kRows - 1) / kRows), kMergeThreads, 0, stream>>>(p);
+  if (p.states <= 2)
+    launch_rows<In, Out, 4>(p, stream);
+  else if (p.states <= 4)
+    launch_rows<In, Out, 2>(p, stream);
+  else
+    launch_rows<In, Out, 1>(p, stream);
 }
 
 }  // namespace

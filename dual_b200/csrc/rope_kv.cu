@@ -32,6 +32,13 @@ __device__ __forceinline__ void unpack8(uint4 w, float* x) {
   x[6] = bf16_lo(w.w); x[7] = bf16_hi(w.w);
 }
 
+// volatile: the load stays where it is written, in front of the position's (q_out may be q, so no .nc)
+__device__ __forceinline__ uint4 ld_row(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 __device__ __forceinline__ uint4 shfl4(uint4 w, int src) {
   w.x = __shfl_sync(0xffffffffu, w.x, src);
   w.y = __shfl_sync(0xffffffffu, w.y, src);
@@ -40,10 +47,17 @@ __device__ __forceinline__ uint4 shfl4(uint4 w, int src) {
   return w;
 }
 
-__global__ void __launch_bounds__(kRopeThreads) rope_set_kv_buffer_kernel(const __grid_constant__ RopeKvParams p) {
+__global__ void __launch_bounds__(kRopeThreads, 5) rope_set_kv_buffer_kernel(const __grid_constant__ RopeKvParams p) {
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
   const int half = lane >> 4, c = lane & 15;  // row of the pair, 16-byte chunk (dims 8c .. 8c + 7)
   for (int64_t i = blockIdx.x; i < p.n; i += gridDim.x) {
+    // the rows' addresses need neither position nor slot: their loads are issued first, so that a token
+    // costs two memory latencies (row and position together, then the table), not three
+    const char* src = part < kQParts ? p.q + i * p.q_stride + part * (kRopeWarpRows * kHeadDim * 2)
+                      : part == kQParts ? p.k + i * p.k_stride : p.v + i * p.v_stride;
+    uint4 raw[kRopeWarpRows / 2];
+#pragma unroll
+    for (int r = 0; r < kRopeWarpRows / 2; ++r) raw[r] = ld_row(src + (2 * r + half) * (kHeadDim * 2) + c * 16);
     const int64_t pos = p.pos64 ? static_cast<const int64_t*>(p.pos)[i] : int64_t(static_cast<const int32_t*>(p.pos)[i]);
     const int64_t slot = p.loc64 ? static_cast<const int64_t*>(p.loc)[i] : int64_t(static_cast<const int32_t*>(p.loc)[i]);
     if (pos < 0 || pos >= p.max_pos) {  // nothing of this token is written
@@ -53,23 +67,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_set_kv_buffer_kernel(const 
     const bool slot_ok = slot >= 0 && slot <= p.capacity;
     if (!slot_ok && threadIdx.x == 0) atomicOr(p.status, kStatusBadLocalSlot);
     if (!slot_ok && part >= kQParts) continue;
-
-    const char* src;
-    char* dst;
-    if (part < kQParts) {
-      src = p.q + i * p.q_stride + part * (kRopeWarpRows * kHeadDim * 2);
-      dst = p.q_out + i * p.q_out_stride + part * (kRopeWarpRows * kHeadDim * 2);
-    } else if (part == kQParts) {
-      src = p.k + i * p.k_stride;
-      dst = p.k_local + slot * p.local_stride;
-    } else {
-      src = p.v + i * p.v_stride;
-      dst = p.v_local + slot * p.local_stride;
-    }
-    uint4 raw[kRopeWarpRows / 2];
-#pragma unroll
-    for (int r = 0; r < kRopeWarpRows / 2; ++r)
-      raw[r] = *reinterpret_cast<const uint4*>(src + (2 * r + half) * (kHeadDim * 2) + c * 16);
+    char* dst = part < kQParts ? p.q_out + i * p.q_out_stride + part * (kRopeWarpRows * kHeadDim * 2)
+                : (part == kQParts ? p.k_local : p.v_local) + slot * p.local_stride;
     if (part > kQParts) {  // v
 #pragma unroll
       for (int r = 0; r < kRopeWarpRows / 2; ++r)

@@ -9,7 +9,7 @@ inside CUDA-graph capture (no host synchronisation, no allocation) except
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Sequence
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -27,6 +27,11 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def _raw_stream(device: int) -> int:
+    """The current stream's handle without a Stream object around it (1-2 us of a call's host time)."""
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _dev(t: torch.Tensor) -> int:
@@ -58,16 +63,22 @@ def default_ctas(device: int = 0) -> int:
 
 def _pool_stride(pool: torch.Tensor, name: str) -> int:
     """Byte stride between consecutive token slots of an NHD page_size-1 plane."""
-    _check(pool.dtype == torch.bfloat16, f"{name} must be bf16")
-    if pool.dim() == 4:  # [pages, page_size=1, heads, dim]
-        _check(pool.shape[1] == 1, f"{name}: page_size must be 1")
-        _check(pool.stride(3) == 1 and pool.stride(2) == HEAD_DIM, f"{name}: heads x dim must be contiguous")
-        _check(tuple(pool.shape[2:]) == (NUM_KV_HEADS, HEAD_DIM), f"{name}: expected 8 kv heads x 128")
+    if pool.dtype is not torch.bfloat16:
+        raise ValueError(f"{name} must be bf16")
+    shape, st = pool.shape, pool.stride()
+    if len(shape) == 4:  # [pages, page_size=1, heads, dim]
+        if shape[1] != 1:
+            raise ValueError(f"{name}: page_size must be 1")
+        if st[2:] != (HEAD_DIM, 1):
+            raise ValueError(f"{name}: heads x dim must be contiguous")
+        if shape[2:] != (NUM_KV_HEADS, HEAD_DIM):
+            raise ValueError(f"{name}: expected 8 kv heads x 128")
     else:
-        _check(pool.dim() == 3 and tuple(pool.shape[1:]) == (NUM_KV_HEADS, HEAD_DIM),
-               f"{name}: expected [slots, 8, 128] or [slots, 1, 8, 128]")
-        _check(pool.stride(2) == 1 and pool.stride(1) == HEAD_DIM, f"{name}: heads x dim must be contiguous")
-    return pool.stride(0) * 2
+        if len(shape) != 3 or shape[1:] != (NUM_KV_HEADS, HEAD_DIM):
+            raise ValueError(f"{name}: expected [slots, 8, 128] or [slots, 1, 8, 128]")
+        if st[1:] != (HEAD_DIM, 1):
+            raise ValueError(f"{name}: heads x dim must be contiguous")
+    return st[0] * 2
 
 
 def tiered_decode(q: torch.Tensor, k_local: torch.Tensor, v_local: torch.Tensor, local_capacity: int,
@@ -224,29 +235,44 @@ def set_kv_buffer(k_local: torch.Tensor, v_local: torch.Tensor, locations: torch
         _stream(k_local.device)))
 
 
-def _on_device(device: torch.device, **tensors: Optional[torch.Tensor]) -> None:
-    for name, t in tensors.items():
-        _check(t is None or t.device == device, f"{name} must be on {device}")
+def _rows(t: torch.Tensor, n: int, heads: int, name: str, device: int) -> Tuple[int, int]:
+    """(pointer, token stride) of ``t``, checked to be bf16 [n, heads, 128] with heads x dims contiguous on ``device``."""
+    st = t.stride()
+    if not (t.dtype is torch.bfloat16 and t.shape == (n, heads, HEAD_DIM) and (n == 0 or st[1:] == (HEAD_DIM, 1))):
+        raise ValueError(f"{name} must be bf16 [n, {heads}, 128] with heads x dims contiguous")
+    if t.get_device() != device:
+        raise ValueError(f"{name} must be on the pools' device")
+    return t.data_ptr(), st[0] if n > 1 else heads * HEAD_DIM  # one token has no stride of its own
 
 
-def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two views [n, heads, dims] share memory: rows at one token stride that lie side by side in
-    one buffer (a fused projection's q | k | v) do not, the same view does."""
-    if a.numel() == 0 or b.numel() == 0:
+def _index(t: torch.Tensor, n: int, name: str, device: int) -> int:
+    """Whether ``t``, checked to be contiguous [n] integers on ``device``, has 64 bits."""
+    if not ((t.dtype is torch.int64 or t.dtype is torch.int32) and t.shape == (n,) and t.is_contiguous()):
+        raise ValueError(f"{name} must be contiguous int64/int32 [n]")
+    if t.get_device() != device:
+        raise ValueError(f"{name} must be on the pools' device")
+    return int(t.dtype is torch.int64)
+
+
+def _weight(t: Optional[torch.Tensor], name: str, device: int) -> Optional[int]:
+    if t is None:
+        return None
+    if not (t.dtype is torch.bfloat16 and t.shape == (HEAD_DIM,) and t.is_contiguous()):
+        raise ValueError(f"{name} must be contiguous bf16 [128]")
+    if t.get_device() != device:
+        raise ValueError(f"{name} must be on the pools' device")
+    return t.data_ptr()
+
+
+def _overlap(a: int, a_step: int, a_size: int, b: int, b_step: int, b_size: int, n: int) -> bool:
+    """Whether n rows of ``a_size`` bytes every ``a_step`` from ``a`` on meet those of ``b``.  Rows at one step
+    that lie side by side (a fused projection's q | k | v) do not."""
+    if a + (n - 1) * a_step + a_size <= b or b + (n - 1) * b_step + b_size <= a:
         return False
-    size = lambda t: t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))  # noqa: E731
-    lo, hi = sorted((a, b), key=lambda t: t.data_ptr())
-    if lo.data_ptr() + size(lo) <= hi.data_ptr():
-        return False
-    step = a.stride(0) * a.element_size()
-    if step and step == b.stride(0) * b.element_size():
-        at = (hi.data_ptr() - lo.data_ptr()) % step
-        return not (size(lo[:1]) <= at and at + size(hi[:1]) <= step)
+    if a_step == b_step and a_step > 0:
+        at = (b - a) % a_step
+        return at < a_size or at + b_size > a_step
     return True
-
-
-def _same_view(a: torch.Tensor, b: torch.Tensor) -> bool:
-    return (a.data_ptr(), a.dtype, a.shape, a.stride()) == (b.data_ptr(), b.dtype, b.shape, b.stride())
 
 
 def rope_set_kv_buffer(k_local: torch.Tensor, v_local: torch.Tensor, locations: torch.Tensor,
@@ -262,37 +288,55 @@ def rope_set_kv_buffer(k_local: torch.Tensor, v_local: torch.Tensor, locations: 
     are free (views of a fused qkv buffer).  Tokens with a bad position are skipped, rows with a bad slot are
     not stored; both are recorded in ``status``."""
     ls = _pool_stride(k_local, "k_local")
-    _check(_pool_stride(v_local, "v_local") == ls and v_local.shape[0] == k_local.shape[0],
-           "k/v local pools must share a slot stride and a size")
+    if not (v_local.shape == k_local.shape and v_local.dtype is k_local.dtype
+            and v_local.stride() == k_local.stride()):
+        raise ValueError("k/v local pools must share a slot stride and a size")
+    dev = k_local.get_device()
     n = locations.numel()
-    for t, heads, name in ((q, NUM_QO_HEADS, "q"), (q_out, NUM_QO_HEADS, "q_out"), (k, NUM_KV_HEADS, "k"),
-                           (v, NUM_KV_HEADS, "v")):
-        _check(t.dtype == torch.bfloat16 and t.dim() == 3 and tuple(t.shape) == (n, heads, HEAD_DIM)
-               and (n == 0 or (t.stride(2) == 1 and t.stride(1) == HEAD_DIM)),
-               f"{name} must be bf16 [n, {heads}, 128] with heads x dims contiguous")
-    for t, name in ((locations, "locations"), (positions, "positions")):
-        _check(t.dtype in (torch.int64, torch.int32) and t.dim() == 1 and t.numel() == n and t.is_contiguous(),
-               f"{name} must be contiguous int64/int32 [n]")
-    _check(cos_sin.dtype == torch.float32 and cos_sin.dim() == 2 and cos_sin.is_contiguous(),
-           "cos_sin must be contiguous fp32 [positions, rotary dims]")
-    for t, name in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
-        _check(t is None or (t.dtype == torch.bfloat16 and tuple(t.shape) == (HEAD_DIM,) and t.is_contiguous()),
-               f"{name} must be contiguous bf16 [128]")
-    _check(status.dtype in (torch.int32, torch.uint32) and status.numel() >= 1, "status must be a 32-bit word")
-    _on_device(k_local.device, v_local=v_local, locations=locations, positions=positions, cos_sin=cos_sin, q=q, k=k,
-               v=v, q_out=q_out, status=status, q_norm_weight=q_norm_weight, k_norm_weight=k_norm_weight)
-    _check(_same_view(q_out, q) or not _overlaps(q_out, q), "q_out must be q itself or not overlap it")
-    _check(not _overlaps(q_out, k) and not _overlaps(q_out, v), "q_out must not overlap k or v")
-    # one token has no stride of its own
-    st = lambda t, heads: t.stride(0) if n > 1 else heads * HEAD_DIM  # noqa: E731
-    lib = _lib.load()
-    _lib.check(lib.dual_rope_set_kv_buffer(
-        k_local.data_ptr(), v_local.data_ptr(), ls, k_local.shape[0] - 1, locations.data_ptr(),
-        int(locations.dtype == torch.int64), positions.data_ptr(), int(positions.dtype == torch.int64),
-        cos_sin.data_ptr(), cos_sin.shape[0], cos_sin.shape[1], int(bool(interleaved)), q.data_ptr(),
-        st(q, NUM_QO_HEADS), k.data_ptr(), st(k, NUM_KV_HEADS), v.data_ptr(), st(v, NUM_KV_HEADS), q_out.data_ptr(),
-        st(q_out, NUM_QO_HEADS), _ptr(q_norm_weight), _ptr(k_norm_weight), float(norm_eps), n, status.data_ptr(),
-        _dev(k_local), _stream(k_local.device)))
+    loc64, pos64 = _index(locations, n, "locations", dev), _index(positions, n, "positions", dev)
+    qp, qs = _rows(q, n, NUM_QO_HEADS, "q", dev)
+    kp, ks = _rows(k, n, NUM_KV_HEADS, "k", dev)
+    vp, vs = _rows(v, n, NUM_KV_HEADS, "v", dev)
+    op, os_ = _rows(q_out, n, NUM_QO_HEADS, "q_out", dev)
+    if not (cos_sin.dtype is torch.float32 and cos_sin.dim() == 2 and cos_sin.is_contiguous()):
+        raise ValueError("cos_sin must be contiguous fp32 [positions, rotary dims]")
+    qw, kw = _weight(q_norm_weight, "q_norm_weight", dev), _weight(k_norm_weight, "k_norm_weight", dev)
+    if not (status.dtype in (torch.int32, torch.uint32) and status.numel() >= 1):
+        raise ValueError("status must be a 32-bit word")
+    if not (v_local.get_device() == cos_sin.get_device() == status.get_device() == dev):
+        raise ValueError("v_local, cos_sin and status must be on the pools' device")
+    q_row, kv_row = NUM_QO_HEADS * HEAD_DIM * 2, NUM_KV_HEADS * HEAD_DIM * 2
+    if (op, os_) != (qp, qs) and _overlap(op, 2 * os_, q_row, qp, 2 * qs, q_row, n):
+        raise ValueError("q_out must be q itself or not overlap it")
+    if (_overlap(op, 2 * os_, q_row, kp, 2 * ks, kv_row, n)
+            or _overlap(op, 2 * os_, q_row, vp, 2 * vs, kv_row, n)):
+        raise ValueError("q_out must not overlap k or v")
+    if dev < 0:
+        raise ValueError(f"expected CUDA tensors, got {k_local.device}")
+    max_pos, rotary = cos_sin.shape
+    _lib.check(_lib.load().dual_rope_set_kv_buffer(
+        k_local.data_ptr(), v_local.data_ptr(), ls, k_local.shape[0] - 1, locations.data_ptr(), loc64,
+        positions.data_ptr(), pos64, cos_sin.data_ptr(), max_pos, rotary, bool(interleaved), qp, qs, kp, ks, vp, vs,
+        op, os_, qw, kw, norm_eps, n, status.data_ptr(), dev, _raw_stream(dev)))
+
+
+def _state(t: torch.Tensor, T: int, name: str, device: int) -> Tuple[int, int, int, int]:
+    """(pointer, token stride, head stride, element size) of an attention state [T, 32, 128]."""
+    st = t.stride()
+    if not ((t.dtype is torch.bfloat16 or t.dtype is torch.float32)
+            and t.shape == (T, NUM_QO_HEADS, HEAD_DIM) and (T == 0 or st[2] == 1)):
+        raise ValueError(f"{name} must be bf16 or fp32 [T, 32, 128] with contiguous head_dim")
+    if t.get_device() != device:
+        raise ValueError(f"{name} must be on out's device")
+    return t.data_ptr(), st[0] if T > 1 else NUM_QO_HEADS * HEAD_DIM, st[1], t.element_size()
+
+
+def _state_lse(t: torch.Tensor, T: int, name: str, device: int) -> int:
+    if not (t.dtype is torch.float32 and t.shape == (T, NUM_QO_HEADS) and t.is_contiguous()):
+        raise ValueError(f"{name} must be contiguous fp32 [T, 32]")
+    if t.get_device() != device:
+        raise ValueError(f"{name} must be on out's device")
+    return t.data_ptr()
 
 
 def merge_attention_states(states: Sequence[torch.Tensor], lses: Sequence[torch.Tensor], out: torch.Tensor,
@@ -301,28 +345,33 @@ def merge_attention_states(states: Sequence[torch.Tensor], lses: Sequence[torch.
     ``run_return_lse`` returns): ``states[i]`` [T, 32, 128], all bf16 or all fp32, ``lses[i]`` fp32 [T, 32]
     (base 2).  ``out`` [T, 32, 128] bf16 or fp32 and ``lse`` [T, 32] (optional) may be one of them."""
     n = len(states)
-    _check(1 <= n <= 8 and len(lses) == n, "need 1 to 8 states, each with its lse")
+    if not (1 <= n <= 8 and len(lses) == n):
+        raise ValueError("need 1 to 8 states, each with its lse")
+    dev = out.get_device()
     T = out.shape[0]
-    for t, name in [(out, "out")] + [(s, f"states[{i}]") for i, s in enumerate(states)]:
-        _check(t.dtype in (torch.bfloat16, torch.float32) and tuple(t.shape) == (T, NUM_QO_HEADS, HEAD_DIM)
-               and (T == 0 or t.stride(2) == 1), f"{name} must be bf16 or fp32 [T, 32, 128] with contiguous head_dim")
-    _check(all(s.dtype == states[0].dtype for s in states), "states must share a type")
-    for t, name in [(lse, "lse")] + [(l, f"lses[{i}]") for i, l in enumerate(lses)]:
-        _check(t is None and name == "lse" or (t.dtype == torch.float32 and tuple(t.shape) == (T, NUM_QO_HEADS)
-                                               and t.is_contiguous()), f"{name} must be contiguous fp32 [T, 32]")
-    _on_device(out.device, lse=lse, **{f"states[{i}]": s for i, s in enumerate(states)},
-               **{f"lses[{i}]": l for i, l in enumerate(lses)})
-    for s in states:
-        _check(_same_view(out, s) or not _overlaps(out, s), "out must be one of the states or not overlap them")
-    for t in lses if lse is not None else ():
-        _check(_same_view(lse, t) or not _overlaps(lse, t), "lse must be one of the lses or not overlap them")
-    arr = lambda vs: (C.c_int64 * n)(*vs)  # noqa: E731
-    st = lambda t: t.stride(0) if T > 1 else NUM_QO_HEADS * HEAD_DIM  # noqa: E731
-    lib = _lib.load()
-    _lib.check(lib.dual_merge_attention_states(
-        _ptrs(states), arr([st(s) for s in states]), arr([s.stride(1) for s in states]), _ptrs(lses), n,
-        int(states[0].dtype == torch.float32), T, out.data_ptr(), st(out), out.stride(1),
-        int(out.dtype == torch.float32), _ptr(lse), _dev(out), _stream(out.device)))
+    op, ot, oh, oe = _state(out, T, "out", dev)
+    if oh < HEAD_DIM or ot < HEAD_DIM:
+        raise ValueError("out must not repeat rows")
+    dtype = states[0].dtype
+    ptrs, toks, heads, lptrs = (C.c_void_p * n)(), (C.c_int64 * n)(), (C.c_int64 * n)(), (C.c_void_p * n)()
+    lp = None if lse is None else _state_lse(lse, T, "lse", dev)
+    for i in range(n):
+        s = states[i]
+        sp, tok, head, e = _state(s, T, f"states[{i}]", dev)
+        if s.dtype is not dtype:
+            raise ValueError("states must share a type")
+        if (sp, tok, head, e) != (op, ot, oh, oe) and _overlap(
+                op, oe * ot, oe * (oh * (NUM_QO_HEADS - 1) + HEAD_DIM), sp, e * tok,
+                e * (head * (NUM_QO_HEADS - 1) + HEAD_DIM), T):
+            raise ValueError("out must be one of the states or not overlap them")
+        l = _state_lse(lses[i], T, f"lses[{i}]", dev)
+        if lp is not None and l != lp and abs(l - lp) < T * NUM_QO_HEADS * 4:
+            raise ValueError("lse must be one of the lses or not overlap them")
+        ptrs[i], toks[i], heads[i], lptrs[i] = sp, tok, head, l
+    if dev < 0:
+        raise ValueError(f"expected CUDA tensors, got {out.device}")
+    _lib.check(_lib.load().dual_merge_attention_states(ptrs, toks, heads, lptrs, n, dtype is torch.float32, T, op, ot,
+                                                       oh, oe == 4, lp, dev, _raw_stream(dev)))
 
 
 def migrate_copy(local_planes: torch.Tensor, remote_planes: torch.Tensor, num_planes: int, num_banks: int,
