@@ -52,6 +52,8 @@ __device__ __forceinline__ void store(__nv_bfloat16* dst, const float* x) {
 }
 
 // R rows per thread and at most kMaxStates / R states: a thread has about eight loads in flight either way.
+// With two states and one row per thread 8,192 tokens took 48 us, with four rows 36; but five tokens took 3.2
+// us instead of 1.9, so rows are spread over threads until every SM has eight blocks.
 template <typename In, typename Out, int R>
 __global__ void __launch_bounds__(kMergeThreads) merge_states_kernel(const __grid_constant__ MergeParams p) {
   constexpr int E = Chunk<In>::kElems, kLanes = kHeadDim / E, kRows = kMergeThreads / kLanes, kStates = kMaxStates / R;
@@ -73,7 +75,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_states_kernel(const __gri
       l[r][s] = p.lse[s][row];
     }
   }
-  __syncthreads();  // every lane of a row has read its log-sum-exps before one of them may be overwritten
+  __syncwarp();  // every lane of a row has read its log-sum-exps before one of them may be overwritten
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     float m = -INFINITY;
@@ -116,9 +118,10 @@ void launch_rows(const MergeParams& p, cudaStream_t stream) {
 
 template <typename In, typename Out>
 void launch(const MergeParams& p, cudaStream_t stream) {
-  if (p.states <= 2)
+  constexpr int64_t kWide = int64_t(148) * 8 * kMergeThreads / (kHeadDim / Chunk<In>::kElems) / kNumQoHeads;  // tokens
+  if (p.states <= 2 && p.tokens >= 4 * kWide)
     launch_rows<In, Out, 4>(p, stream);
-  else if (p.states <= 4)
+  else if (p.states <= 4 && p.tokens >= 2 * kWide)
     launch_rows<In, Out, 2>(p, stream);
   else
     launch_rows<In, Out, 1>(p, stream);

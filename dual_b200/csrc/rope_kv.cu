@@ -20,6 +20,7 @@ constexpr int kRopeWarpRows = 8;                                               /
 constexpr int kRopeParts = (kNumQoHeads + 2 * kNumKvHeads) / kRopeWarpRows;   // warps per token: 6
 constexpr int kQParts = kNumQoHeads / kRopeWarpRows;                          // 4 of them hold q
 constexpr int kRopeThreads = kRopeParts * 32;
+constexpr int kRopeBlocks = 4;                                                // blocks per SM
 static_assert(kNumKvHeads == kRopeWarpRows, "one warp holds a token's k rows, one its v rows");
 
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
@@ -47,19 +48,29 @@ __device__ __forceinline__ uint4 shfl4(uint4 w, int src) {
   return w;
 }
 
-__global__ void __launch_bounds__(kRopeThreads, 5) rope_set_kv_buffer_kernel(const __grid_constant__ RopeKvParams p) {
+__global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_set_kv_buffer_kernel(const __grid_constant__ RopeKvParams p) {
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
   const int half = lane >> 4, c = lane & 15;  // row of the pair, 16-byte chunk (dims 8c .. 8c + 7)
+  const char* const base = part < kQParts ? p.q + part * (kRopeWarpRows * kHeadDim * 2) : part == kQParts ? p.k : p.v;
+  const int64_t stride = part < kQParts ? p.q_stride : part == kQParts ? p.k_stride : p.v_stride;
+  const int64_t lane_off = half * (kHeadDim * 2) + c * 16;
+  uint4 next[kRopeWarpRows / 2];
+  int64_t next_pos = 0, next_slot = 0;
+  // Rows, position and slot of a token are loaded while the token before it is turned: a token then waits
+  // for its table row only.
+  auto fetch = [&](int64_t i) {
+#pragma unroll
+    for (int r = 0; r < kRopeWarpRows / 2; ++r) next[r] = ld_row(base + i * stride + lane_off + r * (kHeadDim * 4));
+    next_pos = p.pos64 ? static_cast<const int64_t*>(p.pos)[i] : int64_t(static_cast<const int32_t*>(p.pos)[i]);
+    next_slot = p.loc64 ? static_cast<const int64_t*>(p.loc)[i] : int64_t(static_cast<const int32_t*>(p.loc)[i]);
+  };
+  fetch(blockIdx.x);  // the grid has at most n blocks
   for (int64_t i = blockIdx.x; i < p.n; i += gridDim.x) {
-    // the rows' addresses need neither position nor slot: their loads are issued first, so that a token
-    // costs two memory latencies (row and position together, then the table), not three
-    const char* src = part < kQParts ? p.q + i * p.q_stride + part * (kRopeWarpRows * kHeadDim * 2)
-                      : part == kQParts ? p.k + i * p.k_stride : p.v + i * p.v_stride;
     uint4 raw[kRopeWarpRows / 2];
 #pragma unroll
-    for (int r = 0; r < kRopeWarpRows / 2; ++r) raw[r] = ld_row(src + (2 * r + half) * (kHeadDim * 2) + c * 16);
-    const int64_t pos = p.pos64 ? static_cast<const int64_t*>(p.pos)[i] : int64_t(static_cast<const int32_t*>(p.pos)[i]);
-    const int64_t slot = p.loc64 ? static_cast<const int64_t*>(p.loc)[i] : int64_t(static_cast<const int32_t*>(p.loc)[i]);
+    for (int r = 0; r < kRopeWarpRows / 2; ++r) raw[r] = next[r];
+    const int64_t pos = next_pos, slot = next_slot;
+    if (i + gridDim.x < p.n) fetch(i + gridDim.x);
     if (pos < 0 || pos >= p.max_pos) {  // nothing of this token is written
       if (threadIdx.x == 0) atomicOr(p.status, kStatusBadPosition);
       continue;
@@ -72,7 +83,7 @@ __global__ void __launch_bounds__(kRopeThreads, 5) rope_set_kv_buffer_kernel(con
     if (part > kQParts) {  // v
 #pragma unroll
       for (int r = 0; r < kRopeWarpRows / 2; ++r)
-        *reinterpret_cast<uint4*>(dst + (2 * r + half) * (kHeadDim * 2) + c * 16) = raw[r];
+        *reinterpret_cast<uint4*>(dst + lane_off + r * (kHeadDim * 4)) = raw[r];
       continue;
     }
 
@@ -141,7 +152,7 @@ __global__ void __launch_bounds__(kRopeThreads, 5) rope_set_kv_buffer_kernel(con
       w.y = pack_bf16x2(o[2], o[3]);
       w.z = pack_bf16x2(o[4], o[5]);
       w.w = pack_bf16x2(o[6], o[7]);
-      *reinterpret_cast<uint4*>(dst + (2 * r + half) * (kHeadDim * 2) + c * 16) = w;
+      *reinterpret_cast<uint4*>(dst + lane_off + r * (kHeadDim * 4)) = w;
     }
   }
 }
@@ -150,7 +161,7 @@ __global__ void __launch_bounds__(kRopeThreads, 5) rope_set_kv_buffer_kernel(con
 
 cudaError_t launch_rope_set_kv_buffer(const RopeKvParams& p, cudaStream_t stream) {
   if (p.n <= 0) return cudaSuccess;
-  const int64_t ctas = p.n < 0x7fffffff ? p.n : 0x7fffffff;
+  const int64_t ctas = p.n < kRopeBlocks * 148 ? p.n : kRopeBlocks * 148;
   rope_set_kv_buffer_kernel<<<int(ctas), kRopeThreads, 0, stream>>>(p);
   return cudaGetLastError();
 }
