@@ -49,6 +49,18 @@ SIGNATURES = {
         VP, C.c_int,                           # status (nullable), num_ctas
         C.c_int, VP]),                         # device, stream
     "dual_decode_noalloc_status": (C.c_int, [U32P, C.c_int, VP]),
+    "dual_shared_prefix_plan": (C.c_int, [VP, VP, C.c_int, C.c_int, VP, C.c_int64, C.POINTER(C.c_int64)]),
+    "dual_shared_prefix_workspace_size": (C.c_int, [VP, C.c_int64, C.POINTER(C.c_size_t)]),
+    "dual_shared_prefix_decode": (C.c_int, [
+        VP, C.c_int64, C.c_int64,              # q, strides
+        VP, VP, C.c_int64, C.c_int64,          # k_local, v_local, local stride, capacity
+        C.POINTER(VP), C.POINTER(VP), C.c_int,  # peer_k, peer_v, num_peers
+        C.c_int64, C.c_int64,                  # peer stride, peer slots
+        VP, C.c_int64, VP, VP, C.c_int64, C.c_int,  # prefix indices, count, indptr, indices, count, batch
+        C.c_double, VP, C.c_int64,             # sm_scale, plan, words
+        VP, C.c_int64, C.c_int64, VP,          # out, strides, lse
+        VP, C.c_size_t, C.c_int,               # workspace, bytes, num_ctas
+        C.c_int, VP]),                         # device, stream
     "dual_append_plan": (C.c_int, [VP, VP, VP, C.c_int, C.c_int, VP, C.c_int64, C.POINTER(C.c_int64)]),
     "dual_tiered_append": (C.c_int, [
         VP, C.c_int64, C.c_int64,              # q, strides

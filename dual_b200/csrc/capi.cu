@@ -4,6 +4,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <string>
 
 #include "dual_b200.h"
@@ -15,6 +16,7 @@
 #include "pack.cuh"
 #include "prefill.cuh"
 #include "rope_kv.cuh"
+#include "shared_prefix.cuh"
 #include "stage.cuh"
 
 namespace {
@@ -165,6 +167,118 @@ int dual_decode_workspace_reset(void* workspace, size_t workspace_bytes, int bat
                                           workspace_bytes);
   DUAL_USE_DEVICE(device);
   DUAL_CHECK_CUDA(cudaMemsetAsync(workspace, 0, head, static_cast<cudaStream_t>(stream)), "workspace reset");
+  return DUAL_OK;
+}
+
+int dual_shared_prefix_plan(const int32_t* group_indptr_host, const int32_t* prefix_indptr_host, int groups,
+                            int num_ctas, int32_t* plan_host, int64_t max_words, int64_t* num_words) {
+  g_last_error.clear();
+  if (groups < 0 || num_ctas <= 0 || num_ctas > 65535 || !num_words)
+    return fail(DUAL_EINVAL, "bad shared-prefix plan arguments");
+  if (groups > 0 && (!group_indptr_host || !prefix_indptr_host)) return fail(DUAL_EINVAL, "null indptr");
+  for (int g = 0; g < groups; ++g)
+    if (group_indptr_host[g] > group_indptr_host[g + 1] || prefix_indptr_host[g] > prefix_indptr_host[g + 1])
+      return fail(DUAL_EINVAL, "group %d: negative length", g);
+  if (groups > 0 && (group_indptr_host[0] != 0 || prefix_indptr_host[0] != 0))
+    return fail(DUAL_EINVAL, "group_indptr and prefix_indptr start at 0");
+  try {
+    *num_words = dual::shared_prefix_plan(group_indptr_host, prefix_indptr_host, groups, num_ctas, plan_host, max_words);
+  } catch (const std::exception& e) {
+    return fail(DUAL_ENOSPACE, "shared-prefix plan: %s", e.what());
+  }
+  return DUAL_OK;
+}
+
+int dual_shared_prefix_workspace_size(const int32_t* plan_host, int64_t plan_words, size_t* bytes) {
+  g_last_error.clear();
+  dual::PlanView plan;
+  if (!plan_host || !bytes || !plan.open(plan_host, plan_words)) return fail(DUAL_EINVAL, "not a shared-prefix plan");
+  *bytes = dual::decode_workspace_bytes(plan.requests, plan.ctas) + size_t(plan.state_size) * 16;
+  return DUAL_OK;
+}
+
+int dual_shared_prefix_decode(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_local,
+                              const void* v_local, int64_t local_stride_bytes, int64_t local_capacity,
+                              const void* const* peer_k, const void* const* peer_v, int num_peers,
+                              int64_t peer_stride_bytes, int64_t peer_slots, const int32_t* prefix_indices,
+                              int64_t num_prefix_indices, const int32_t* kv_indptr, const int32_t* unified_indices,
+                              int64_t num_indices, int batch, double sm_scale, const int32_t* plan, int64_t plan_words,
+                              void* out, int64_t out_stride_token, int64_t out_stride_head, float* lse,
+                              void* workspace, size_t workspace_bytes, int num_ctas, int device, void* stream) {
+  g_last_error.clear();
+  if (batch < 0) return fail(DUAL_EINVAL, "batch must be >= 0 (got %d)", batch);
+  if (batch == 0) return DUAL_OK;
+  if (!q || !k_local || !v_local || !kv_indptr || !plan || !out || !workspace)
+    return fail(DUAL_EINVAL, "null pointer argument");
+  if ((num_prefix_indices > 0 && !prefix_indices) || (num_indices > 0 && !unified_indices))
+    return fail(DUAL_EINVAL, "null index list");
+  if (num_peers < 0 || num_peers > dual::kMaxPeers)
+    return fail(DUAL_EINVAL, "num_peers must be in [0, %d] (got %d)", dual::kMaxPeers, num_peers);
+  const int64_t min_stride = int64_t(dual::kNumKvHeads) * dual::kHeadDim * 2;
+  if (!aligned16(k_local) || !aligned16(v_local) || (local_stride_bytes & 15) || local_stride_bytes < min_stride)
+    return fail(DUAL_EINVAL, "local pool must be 16-byte aligned with a slot stride >= 2048 B, multiple of 16");
+  if (local_capacity < 0 || local_capacity > 0xfffffffeLL) return fail(DUAL_EINVAL, "local_capacity out of range");
+  if ((q_stride_head % 8) || (q_stride_token % 8) || (out_stride_head % 8) || (out_stride_token % 8) ||
+      !aligned16(q) || !aligned16(out))
+    return fail(DUAL_EINVAL, "q/out must be 16-byte aligned with element strides that are multiples of 8");
+  if (num_peers > 0) {
+    if (!peer_k || !peer_v) return fail(DUAL_EINVAL, "peer pointer arrays are null");
+    if ((peer_stride_bytes & 15) || peer_stride_bytes < min_stride || peer_slots <= 0)
+      return fail(DUAL_EINVAL, "peer banks need a 16-byte multiple slot stride >= 2048 B and slots > 0");
+    for (int i = 0; i < num_peers; ++i)
+      if (!peer_k[i] || !peer_v[i] || !aligned16(peer_k[i]) || !aligned16(peer_v[i]))
+        return fail(DUAL_EINVAL, "peer bank %d pointer null or not 16-byte aligned", i);
+  }
+  if (!(sm_scale > 0.0)) return fail(DUAL_EINVAL, "sm_scale must be positive");
+  if (plan_words < dual::kPlanHeader || !aligned16(plan)) return fail(DUAL_EINVAL, "plan must be a 16-byte aligned plan");
+  if (num_ctas <= 0 || num_ctas > 65535) return fail(DUAL_EINVAL, "num_ctas must be the plan's");
+  const size_t own = dual::decode_workspace_bytes(batch, num_ctas);
+  if (workspace_bytes < own)
+    return fail(DUAL_ENOSPACE, "workspace too small: need more than %zu bytes, got %zu", own, workspace_bytes);
+  if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(DUAL_EINVAL, "workspace must be 256-byte aligned");
+  DUAL_USE_DEVICE(device);
+
+  dual::SharedPrefixParams s{};
+  dual::SharedDecodeParams p{};
+  s.q = p.q = static_cast<const __nv_bfloat16*>(q);
+  s.q_stride_tok = p.q_stride_tok = q_stride_token;
+  s.q_stride_head = p.q_stride_head = q_stride_head;
+  s.k_local = p.k_local = static_cast<const char*>(k_local);
+  s.v_local = p.v_local = static_cast<const char*>(v_local);
+  s.local_stride = p.local_stride = local_stride_bytes;
+  s.local_capacity = p.local_capacity = local_capacity;
+  for (int i = 0; i < dual::kMaxPeers; ++i) {
+    s.peer_k[i] = p.peer_k[i] = i < num_peers ? static_cast<const char*>(peer_k[i]) : nullptr;
+    s.peer_v[i] = p.peer_v[i] = i < num_peers ? static_cast<const char*>(peer_v[i]) : nullptr;
+  }
+  s.num_peers = p.num_peers = num_peers;
+  s.peer_stride = p.peer_stride = peer_stride_bytes;
+  s.peer_slots = p.peer_slots = peer_slots;
+  s.batch = p.batch = batch;
+  s.scale_log2 = p.scale_log2 = static_cast<float>(sm_scale * 1.4426950408889634);
+  s.status = p.status = static_cast<unsigned*>(workspace);
+  s.plan = p.plan = plan;
+  s.plan_words = p.plan_words = plan_words;
+  s.ctas = p.grid_g = num_ctas;
+  s.indices = prefix_indices;
+  s.num_indices = num_prefix_indices < 0 ? 0 : num_prefix_indices;
+  char* const states = static_cast<char*>(workspace) + own;
+  s.states = reinterpret_cast<float*>(states);
+  p.states = reinterpret_cast<const float4*>(states);
+  s.state_size = p.state_size = int64_t((workspace_bytes - own) / 16);
+  p.indptr = kv_indptr;
+  p.indices = unified_indices;
+  p.num_indices = num_indices < 0 ? 0 : num_indices;
+  p.counters = reinterpret_cast<unsigned*>(static_cast<char*>(workspace) + 256);
+  p.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + dual::decode_workspace_head_bytes(batch));
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.out_stride_tok = out_stride_token;
+  p.out_stride_head = out_stride_head;
+  p.lse = lse;
+  cudaError_t e = dual::launch_shared_prefix(s, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "shared prefix launch");
+  e = dual::launch_shared_decode(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "shared prefix decode launch");
   return DUAL_OK;
 }
 

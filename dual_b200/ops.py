@@ -123,6 +123,97 @@ def tiered_decode(q: torch.Tensor, k_local: torch.Tensor, v_local: torch.Tensor,
         dev, _stream(q.device)))
 
 
+def _host_indptr(t, name: str) -> torch.Tensor:
+    t = torch.as_tensor(t)
+    if t.dim() != 1 or t.numel() < 1 or t.is_floating_point():
+        raise ValueError(f"{name} must be a list of integers [groups + 1]")
+    return t.to("cpu", torch.int32).contiguous()
+
+
+def shared_prefix_plan(group_indptr, prefix_indptr, num_ctas: int = 0) -> torch.Tensor:
+    """Host-side work plan of a decode with shared prefixes, an int32 CPU tensor: requests
+    ``group_indptr[g] .. group_indptr[g + 1]`` share the prefix of ``prefix_indptr[g + 1] - prefix_indptr[g]``
+    entries.  It stays valid while both do.  ``group_indptr`` / ``prefix_indptr``: host sequences or tensors."""
+    gi, pi = _host_indptr(group_indptr, "group_indptr"), _host_indptr(prefix_indptr, "prefix_indptr")
+    if gi.numel() != pi.numel():
+        raise ValueError("group_indptr and prefix_indptr need one entry per group and one more")
+    groups, ctas = gi.numel() - 1, int(num_ctas) or default_ctas(0)
+    lib = _lib.load()
+    n = C.c_int64(0)
+    _lib.check(lib.dual_shared_prefix_plan(gi.data_ptr(), pi.data_ptr(), groups, ctas, None, 0, C.byref(n)))
+    plan = torch.empty(n.value, dtype=torch.int32)
+    _lib.check(lib.dual_shared_prefix_plan(gi.data_ptr(), pi.data_ptr(), groups, ctas, plan.data_ptr(), n.value,
+                                           C.byref(n)))
+    return plan
+
+
+def shared_prefix_workspace_size(plan: torch.Tensor) -> int:
+    """Workspace bytes of a call with this (host) plan."""
+    if plan.device.type != "cpu" or plan.dtype is not torch.int32 or not plan.is_contiguous():
+        raise ValueError("plan must be a host plan of shared_prefix_plan")
+    n = C.c_size_t(0)
+    _lib.check(_lib.load().dual_shared_prefix_workspace_size(plan.data_ptr(), plan.numel(), C.byref(n)))
+    return int(n.value)
+
+
+def shared_prefix_decode(q: torch.Tensor, k_local: torch.Tensor, v_local: torch.Tensor, local_capacity: int,
+                         peer_k: Sequence[torch.Tensor], peer_v: Sequence[torch.Tensor],
+                         prefix_indices: torch.Tensor, kv_indptr: torch.Tensor, unified_indices: torch.Tensor,
+                         sm_scale: float, plan: torch.Tensor, out: torch.Tensor, lse: Optional[torch.Tensor],
+                         workspace: torch.Tensor, num_ctas: int = 0) -> None:
+    """One decode layer of a batch in groups that share prefixes: request b sees its group's part of
+    ``prefix_indices`` and its own entries ``unified_indices[kv_indptr[b] .. kv_indptr[b + 1]]``.  ``plan``: that of
+    ``shared_prefix_plan`` on the device.  ``workspace``: ``shared_prefix_workspace_size`` bytes, its head zeroed once
+    with ``decode_workspace_reset``; the status word is its first."""
+    dev = q.get_device()
+    B = q.shape[0]
+    qt, ot = q.stride(), out.stride()
+    if q.dtype is not torch.bfloat16 or q.shape != (B, NUM_QO_HEADS, HEAD_DIM) or qt[2] != 1:
+        raise ValueError("q must be bf16 [B, 32, 128] with contiguous head_dim")
+    if out.dtype is not torch.bfloat16 or out.shape != q.shape or ot[2] != 1:
+        raise ValueError("out must be bf16 [B, 32, 128] with contiguous head_dim")
+    for t, name in ((kv_indptr, "kv_indptr"), (prefix_indices, "prefix_indices"), (unified_indices, "unified_indices"),
+                    (plan, "plan")):
+        if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.get_device() != dev:
+            raise ValueError(f"{name} must be contiguous int32 [n] on q's device")
+    if kv_indptr.numel() < B + 1:
+        raise ValueError("kv_indptr too short")
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (B, NUM_QO_HEADS) or not lse.is_contiguous()
+                            or lse.get_device() != dev):
+        raise ValueError("lse must be contiguous fp32 [B, 32] on q's device")
+    ls = _pool_stride(k_local, "k_local")
+    if v_local.shape != k_local.shape or v_local.dtype is not k_local.dtype or v_local.stride() != k_local.stride():
+        raise ValueError("k/v local pools must share a slot stride and a size")
+    if not 0 <= local_capacity < k_local.shape[0]:
+        raise ValueError("local_capacity must be a slot of the local pools")
+    if not out.get_device() == k_local.get_device() == v_local.get_device() == workspace.get_device() == dev:
+        raise ValueError("out, the pools and the workspace must be on q's device")
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    n = len(peer_k)
+    if len(peer_v) != n:
+        raise ValueError("peer_k / peer_v count mismatch")
+    pk, pv, ps, slots = (C.c_void_p * max(n, 1))(), (C.c_void_p * max(n, 1))(), 0, 0
+    if n > 8:
+        raise ValueError("at most 8 supplier banks")
+    if n:
+        ps, slots = _pool_stride(peer_k[0], "peer_k0"), peer_k[0].shape[0]
+        for i in range(n):
+            for t, name in ((peer_k[i], "peer_k"), (peer_v[i], "peer_v")):
+                if t.shape[0] != slots or _pool_stride(t, name) != ps or t.get_device() < 0:
+                    raise ValueError(f"{name}{i}: all supplier banks must share a size and a slot stride, on GPUs")
+            pk[i], pv[i] = peer_k[i].data_ptr(), peer_v[i].data_ptr()
+    if dev < 0:
+        raise ValueError(f"expected CUDA tensors, got {q.device}")
+    _lib.check(_lib.load().dual_shared_prefix_decode(
+        q.data_ptr(), qt[0] if B > 1 else NUM_QO_HEADS * HEAD_DIM, qt[1], k_local.data_ptr(), v_local.data_ptr(), ls,
+        local_capacity, pk, pv, n, ps, slots, prefix_indices.data_ptr(), prefix_indices.numel(), kv_indptr.data_ptr(),
+        unified_indices.data_ptr(), unified_indices.numel(), B, sm_scale, plan.data_ptr(), plan.numel(), out.data_ptr(),
+        ot[0] if B > 1 else NUM_QO_HEADS * HEAD_DIM, ot[1], None if lse is None else lse.data_ptr(),
+        workspace.data_ptr(), workspace.numel() * workspace.element_size(), num_ctas or default_ctas(dev), dev,
+        _raw_stream(dev)))
+
+
 def append_plan(qo_indptr, kv_indptr, causal: bool, remote_counts=None) -> torch.Tensor:
     """Host-side work list (request, kv head, 64-token query pair, kv tiles it sees), grouped by
     (request, kv head), longest groups first and pairs longest first, as an int32 CPU tensor [n, 4].

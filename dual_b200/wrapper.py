@@ -137,6 +137,109 @@ class BatchDecodeWithPagedKVCacheWrapper:
     run_return_lse = functools.partialmethod(run, return_lse=True)
 
 
+class SharedPrefixDecodeWrapper:
+    """Decode of a batch whose requests share prefixes, by ``BatchDecodeWithPagedKVCacheWrapper``'s convention.
+
+    Requests ``group_indptr[g] .. group_indptr[g + 1]`` share the prefix
+    ``prefix_indices[prefix_indptr[g] .. prefix_indptr[g + 1]]`` and have entries of their own, ``indices`` by
+    ``indptr``.  ``plan`` is called once per step (it builds the work plan of the prefixes on the host) and ``run``
+    once per layer.  For CUDA graphs pass ``use_cuda_graph=True`` and the buffers that ``plan`` shall fill: the
+    captured ``run`` reads them again at every replay.
+    """
+
+    def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD", use_cuda_graph: bool = False,
+                 paged_kv_indptr_buffer: Optional[torch.Tensor] = None,
+                 paged_kv_indices_buffer: Optional[torch.Tensor] = None,
+                 prefix_indices_buffer: Optional[torch.Tensor] = None, plan_buffer: Optional[torch.Tensor] = None,
+                 num_ctas: int = 0):
+        if kv_layout != "NHD":
+            raise ValueError("only the NHD layout is supported")
+        self._use_cuda_graph = use_cuda_graph
+        self.device = float_workspace_buffer.device
+        self._float_workspace = float_workspace_buffer
+        self._num_ctas = num_ctas or ops.default_ctas(self.device.index or 0)
+        self._buffers = dict(indptr=paged_kv_indptr_buffer, indices=paged_kv_indices_buffer,
+                             prefix=prefix_indices_buffer, plan=plan_buffer)
+        for name, t in self._buffers.items():
+            if use_cuda_graph and (t is None or t.dtype != torch.int32 or t.device != self.device):
+                raise ValueError(f"CUDA graphs need an int32 {name} buffer on {self.device}")
+        self._batch = None
+        self._sm_scale = None
+
+    def _fill(self, name: str, values: torch.Tensor, non_blocking: bool) -> torch.Tensor:
+        """``values`` in the buffer ``name``: the part that holds them, or with CUDA graphs the whole buffer."""
+        n = values.numel()
+        buf = self._buffers[name]
+        if buf is None or buf.numel() < n:
+            if self._use_cuda_graph:
+                raise ValueError(f"{n} words exceed the CUDA-graph {name} buffer")
+            buf = self._buffers[name] = torch.empty(max(n, 1), dtype=torch.int32, device=self.device)
+        buf[:n].copy_(values.to(torch.int32), non_blocking=non_blocking)
+        return buf if self._use_cuda_graph else buf[:n]
+
+    def plan(self, group_indptr, prefix_indptr, prefix_indices: torch.Tensor, indptr: torch.Tensor,
+             indices: torch.Tensor, num_qo_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
+             sm_scale: Optional[float] = None, non_blocking: bool = True) -> None:
+        """``group_indptr`` / ``prefix_indptr`` (host sequences or tensors) are read on the host; the index lists
+        and ``indptr`` are copied to the device."""
+        if (num_qo_heads, num_kv_heads, head_dim, page_size) != (ops.NUM_QO_HEADS, ops.NUM_KV_HEADS,
+                                                                 ops.HEAD_DIM, 1):
+            raise ValueError("dual_b200 decode is built for 32 q heads, 8 kv heads, head_dim 128, page_size 1")
+        gi, pi = torch.as_tensor(group_indptr).to("cpu"), torch.as_tensor(prefix_indptr).to("cpu")
+        words = ops.shared_prefix_plan(gi, pi, self._num_ctas)
+        batch = int(gi[-1])
+        if indptr.numel() != batch + 1:
+            raise ValueError(f"indptr is for {indptr.numel() - 1} requests, the groups hold {batch}")
+        if prefix_indices.numel() < int(pi[-1]):
+            raise ValueError("prefix_indices is shorter than the prefixes")
+        if self._use_cuda_graph and self._batch not in (None, batch):
+            raise ValueError(f"CUDA graphs keep their batch: {self._batch}, got {batch}")
+        need = ops.shared_prefix_workspace_size(words)
+        if self._float_workspace.numel() * self._float_workspace.element_size() < need:
+            raise ValueError(f"float_workspace_buffer too small: need {need} bytes")
+        self._plan = self._fill("plan", words, non_blocking)
+        self._prefix = self._fill("prefix", prefix_indices, non_blocking)
+        self._indptr = self._fill("indptr", indptr, non_blocking)
+        self._indices = self._fill("indices", indices, non_blocking)
+        # the caller's buffer may hold anything: zero the status word and the kernels' arrival counters
+        ops.decode_workspace_reset(self._float_workspace, batch)
+        self._batch = batch
+        self._sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(head_dim)
+
+    def run(self, q: torch.Tensor, paged_kv_cache, *args, out: Optional[torch.Tensor] = None,
+            lse: Optional[torch.Tensor] = None, return_lse: bool = False):
+        """``run(q, paged_kv)`` over the planned lists, all local, or the tiered form ``run(q, paged_kv, *[peer_k_i,
+        peer_v_i], prefix_indices, unified_indices, local_capacity, sm_scale)``."""
+        B = self._batch
+        if B is None:
+            raise RuntimeError("plan() must be called before run()")
+        k, v = _unpack_paged_kv(paged_kv_cache)
+        if args:
+            if len(args) < 4 or len(args) % 2:
+                raise ValueError("tiered run expects (*[peer_k_i, peer_v_i], prefix_indices, unified_indices, "
+                                 "local_capacity, sm_scale)")
+            peer_k, peer_v = args[:-4:2], args[1:-4:2]
+            prefix, indices, capacity, scale = args[-4:]
+        else:
+            peer_k, peer_v = (), ()
+            prefix, indices, capacity, scale = self._prefix, self._indices, k.shape[0] - 1, self._sm_scale
+        if q.shape[0] != B:
+            raise ValueError(f"q has {q.shape[0]} rows but plan() was for batch {B}")
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        if return_lse and lse is None:
+            lse = torch.empty((B, ops.NUM_QO_HEADS), dtype=torch.float32, device=q.device)
+        ops.shared_prefix_decode(q, k, v, int(capacity), peer_k, peer_v, prefix, self._indptr, indices, float(scale),
+                                 self._plan, out, lse if return_lse else None, self._float_workspace, self._num_ctas)
+        return (out, lse) if return_lse else out
+
+    run_return_lse = functools.partialmethod(run, return_lse=True)
+
+    def status(self) -> int:
+        """Device status bits of this wrapper's launches since the last ``plan`` (synchronous read)."""
+        return ops.status_read(self._float_workspace)
+
+
 class BatchPrefillWithPagedKVCacheWrapper:
     """Paged append / prefill attention (page_size 1, NHD), FlashInfer's plan/run convention.
 

@@ -123,6 +123,39 @@ int dual_tiered_decode_noalloc(const void* q, int64_t q_stride_token, int64_t q_
  * Synchronous (not capturable); allocates nothing. */
 int dual_decode_noalloc_status(uint32_t* value_out, int device, void* stream);
 
+/* ------------------------------------------- decode with shared prefixes ---
+ * Decode of a batch whose requests share prefixes (a system prompt, a document, the samples of one
+ * prompt; no counterpart in the reference).  Requests group_indptr[g] .. group_indptr[g+1)-1 are group g
+ * and share the prefix list prefix_indices[prefix_indptr[g] .. prefix_indptr[g+1)); request b besides
+ * has its own list unified_indices[kv_indptr[b] .. kv_indptr[b+1)), as in dual_tiered_decode:
+ *   out_b = softmax(sm_scale q_b [K_prefix; K_own]^T) [V_prefix; V_own],   lse base 2.
+ * Any list may be empty; where both are, out = 0 and lse = -inf.  Equal to dual_tiered_decode over the
+ * concatenated lists, but a prefix is read once per 64 requests, not once per request.
+ *
+ * dual_shared_prefix_plan (host): from HOST copies of group_indptr and prefix_indptr ([groups + 1],
+ * starting at 0; group_indptr[groups] is the batch), writes the work plan (int32 words) and returns its
+ * size in *num_words (call with plan_host = NULL to size it).  The plan is copied to the device (16-byte
+ * aligned) and stays valid while the groups and the prefixes' lengths do: a decode loop that appends to
+ * the requests' own lists makes it once.  num_ctas: CTAs of both launches (dual_decode_default_ctas).
+ * dual_shared_prefix_workspace_size (host): bytes that a call with this plan needs; a larger workspace
+ * serves smaller plans.  The workspace is the decode workspace followed by the prefixes' states: zero its
+ * head once with dual_decode_workspace_reset (its counters stand behind the status word as there).
+ * dual_shared_prefix_decode: two launches, the second started as the first ends.  A plan that does not
+ * fit the call (another batch, num_ctas or index list, a workspace too small for it) records
+ * DUAL_STATUS_BAD_LENGTH; the outputs are then not to be used.  Calls that share a workspace must not
+ * overlap.  q, out: 16-byte aligned, element strides that are multiples of 8. */
+int dual_shared_prefix_plan(const int32_t* group_indptr_host, const int32_t* prefix_indptr_host, int groups,
+                            int num_ctas, int32_t* plan_host, int64_t max_words, int64_t* num_words);
+int dual_shared_prefix_workspace_size(const int32_t* plan_host, int64_t plan_words, size_t* bytes);
+int dual_shared_prefix_decode(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_local,
+                              const void* v_local, int64_t local_stride_bytes, int64_t local_capacity,
+                              const void* const* peer_k, const void* const* peer_v, int num_peers,
+                              int64_t peer_stride_bytes, int64_t peer_slots, const int32_t* prefix_indices,
+                              int64_t num_prefix_indices, const int32_t* kv_indptr, const int32_t* unified_indices,
+                              int64_t num_indices, int batch, double sm_scale, const int32_t* plan, int64_t plan_words,
+                              void* out, int64_t out_stride_token, int64_t out_stride_head, float* lse,
+                              void* workspace, size_t workspace_bytes, int num_ctas, int device, void* stream);
+
 /* ------------------------------------------------------ tiered append ---
  * Replaces the tiered FA2 batch-prefill module on the append path (run hook
  * peer/prefill_backend.py:25-42, module peer/flashinfer_peer.py:105-142).  The banks passed as
