@@ -193,7 +193,7 @@ int dual_shared_prefix_workspace_size(const int32_t* plan_host, int64_t plan_wor
   g_last_error.clear();
   dual::PlanView plan;
   if (!plan_host || !bytes || !plan.open(plan_host, plan_words)) return fail(DUAL_EINVAL, "not a shared-prefix plan");
-  *bytes = dual::decode_workspace_bytes(plan.requests, plan.ctas) + size_t(plan.state_size) * 16;
+  *bytes = 256 + dual::shared_prefix_own_bytes(plan.requests, plan.ctas) + size_t(plan.state_size) * 16;
   return DUAL_OK;
 }
 
@@ -232,52 +232,46 @@ int dual_shared_prefix_decode(const void* q, int64_t q_stride_token, int64_t q_s
   if (!(sm_scale > 0.0)) return fail(DUAL_EINVAL, "sm_scale must be positive");
   if (plan_words < dual::kPlanHeader || !aligned16(plan)) return fail(DUAL_EINVAL, "plan must be a 16-byte aligned plan");
   if (num_ctas <= 0 || num_ctas > 65535) return fail(DUAL_EINVAL, "num_ctas must be the plan's");
-  const size_t own = dual::decode_workspace_bytes(batch, num_ctas);
-  if (workspace_bytes < own)
-    return fail(DUAL_ENOSPACE, "workspace too small: need more than %zu bytes, got %zu", own, workspace_bytes);
+  const size_t head = 256 + dual::shared_prefix_own_bytes(batch, num_ctas);
+  if (workspace_bytes < head)
+    return fail(DUAL_ENOSPACE, "workspace too small: need at least %zu bytes, got %zu", head, workspace_bytes);
   if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(DUAL_EINVAL, "workspace must be 256-byte aligned");
   DUAL_USE_DEVICE(device);
 
-  dual::SharedPrefixParams s{};
-  dual::SharedDecodeParams p{};
-  s.q = p.q = static_cast<const __nv_bfloat16*>(q);
-  s.q_stride_tok = p.q_stride_tok = q_stride_token;
-  s.q_stride_head = p.q_stride_head = q_stride_head;
-  s.k_local = p.k_local = static_cast<const char*>(k_local);
-  s.v_local = p.v_local = static_cast<const char*>(v_local);
-  s.local_stride = p.local_stride = local_stride_bytes;
-  s.local_capacity = p.local_capacity = local_capacity;
+  dual::SharedPrefixParams p{};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_stride_tok = q_stride_token;
+  p.q_stride_head = q_stride_head;
+  p.k_local = static_cast<const char*>(k_local);
+  p.v_local = static_cast<const char*>(v_local);
+  p.local_stride = local_stride_bytes;
+  p.local_capacity = local_capacity;
   for (int i = 0; i < dual::kMaxPeers; ++i) {
-    s.peer_k[i] = p.peer_k[i] = i < num_peers ? static_cast<const char*>(peer_k[i]) : nullptr;
-    s.peer_v[i] = p.peer_v[i] = i < num_peers ? static_cast<const char*>(peer_v[i]) : nullptr;
+    p.peer_k[i] = i < num_peers ? static_cast<const char*>(peer_k[i]) : nullptr;
+    p.peer_v[i] = i < num_peers ? static_cast<const char*>(peer_v[i]) : nullptr;
   }
-  s.num_peers = p.num_peers = num_peers;
-  s.peer_stride = p.peer_stride = peer_stride_bytes;
-  s.peer_slots = p.peer_slots = peer_slots;
-  s.batch = p.batch = batch;
-  s.scale_log2 = p.scale_log2 = static_cast<float>(sm_scale * 1.4426950408889634);
-  s.status = p.status = static_cast<unsigned*>(workspace);
-  s.plan = p.plan = plan;
-  s.plan_words = p.plan_words = plan_words;
-  s.ctas = p.grid_g = num_ctas;
-  s.indices = prefix_indices;
-  s.num_indices = num_prefix_indices < 0 ? 0 : num_prefix_indices;
-  char* const states = static_cast<char*>(workspace) + own;
-  s.states = reinterpret_cast<float*>(states);
-  p.states = reinterpret_cast<const float4*>(states);
-  s.state_size = p.state_size = int64_t((workspace_bytes - own) / 16);
+  p.num_peers = num_peers;
+  p.peer_stride = peer_stride_bytes;
+  p.peer_slots = peer_slots;
+  p.prefix = prefix_indices;
+  p.num_prefix = num_prefix_indices < 0 ? 0 : num_prefix_indices;
   p.indptr = kv_indptr;
   p.indices = unified_indices;
   p.num_indices = num_indices < 0 ? 0 : num_indices;
-  p.counters = reinterpret_cast<unsigned*>(static_cast<char*>(workspace) + 256);
-  p.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + dual::decode_workspace_head_bytes(batch));
+  p.batch = batch;
+  p.scale_log2 = static_cast<float>(sm_scale * 1.4426950408889634);
+  p.plan = plan;
+  p.plan_words = plan_words;
+  p.status = static_cast<unsigned*>(workspace);
+  p.own = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+  p.states = reinterpret_cast<float*>(static_cast<char*>(workspace) + head);
+  p.state_size = int64_t((workspace_bytes - head) / 16);
+  p.ctas = num_ctas;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.out_stride_tok = out_stride_token;
   p.out_stride_head = out_stride_head;
   p.lse = lse;
-  cudaError_t e = dual::launch_shared_prefix(s, static_cast<cudaStream_t>(stream));
-  if (e != cudaSuccess) return cuda_fail(e, "shared prefix launch");
-  e = dual::launch_shared_decode(p, static_cast<cudaStream_t>(stream));
+  cudaError_t e = dual::launch_shared_prefix_decode(p, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "shared prefix decode launch");
   return DUAL_OK;
 }

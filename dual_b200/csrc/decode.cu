@@ -1,8 +1,5 @@
 // Tiered split-KV paged decode kernel + partial-state merge (see decode.cuh).
-#include <type_traits>
-
 #include "decode.cuh"
-#include "shared_prefix.cuh"
 
 namespace dual {
 namespace {
@@ -123,94 +120,8 @@ __device__ __noinline__ void merge_request_heads(const TieredDecodeParams& p, co
   }
 }
 
-// A partial state of the requests' own entries beside a shared prefix: the layout of the prefix's states with
-// the four rows of one request, at (segment, kv head).
-constexpr int kOwnState = kStateGroups * kGqa;  // 16-byte units
-static_assert(kOwnState * 4 == kGqa * kPartialStride, "one workspace formula for both layouts");
-
-// Join the states of request b's own entries (CTAs glo..ghi, none when glo > ghi) and of its group's prefix for
-// the 4 q heads of kv head h (one warp) and write the bf16 output and the base-2 LSE.  Lane = (row lane % 4,
-// column groups lane / 4 + 8 k), so that four lanes read 64 consecutive bytes; the maximum is found first,
-// eight states at a time.
-__device__ __noinline__ void merge_shared_prefix(const SharedDecodeParams& p, const Split& sp, int b, int h, int glo,
-                                                 int ghi, int lane) {
-  const int r = lane & 3, cg = lane >> 2;
-  const float4* own = reinterpret_cast<const float4*>(p.partial) + (int64_t(b) * kNumKvHeads + h) * kOwnState + r;
-  constexpr int64_t kOwnSeg = int64_t(kNumKvHeads) * kOwnState;
-  const float4* pre = p.states;
-  int n_pre = 0;
-  int64_t pitch = 0;
-  PlanView plan;
-  bool ok = plan.open(p.plan, p.plan_words) && plan.requests == p.batch;
-  if (ok) {
-    const int2 req = __ldg(reinterpret_cast<const int2*>(plan.words + plan.request_at()) + b);
-    if (req.x >= 0) {
-      ok = req.x < plan.blocks;
-      const int4 job = ok ? __ldg(reinterpret_cast<const int4*>(plan.words + plan.job_at()) + req.x * kNumKvHeads + h)
-                          : make_int4(0, 0, 0, 0);
-      const int64_t off = uint32_t(job.x);
-      pitch = int64_t(kGqa) * job.z;
-      ok = ok && job.y >= 0 && job.z > 0 && job.z <= kBlockRequests && req.y >= 0 && req.y < job.z &&
-           off + int64_t(job.y) * kStateGroups * pitch <= p.state_size;
-      if (ok) {
-        pre += off + kGqa * req.y + r;
-        n_pre = job.y;
-      }
-    }
-  }
-  if (!ok && lane == 0) atomicOr(p.status, kStatusBadLength);
-  const int64_t pre_seg = kStateGroups * pitch;
-
-  float M = -INFINITY;
-  for (int i = cg; i < n_pre; i += 8) M = fmaxf(M, __ldcg(&pre[i * pre_seg + (kStateGroups - 1) * pitch].x));
-  for (int gg = glo + cg; gg <= ghi; gg += 8)
-    if (sp.nonempty(gg)) M = fmaxf(M, __ldcg(&own[gg * kOwnSeg + (kStateGroups - 1) * kGqa].x));
-#pragma unroll
-  for (int d = 4; d <= 16; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-  float D = 0.f;
-  float4 acc[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](const float4* state, int64_t step) {
-    const float4 md = __ldcg(state + (kStateGroups - 1) * step);
-    float4 v[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = __ldcg(state + (cg + 8 * k) * step);
-    const float w = md.x == -INFINITY ? 0.f : exp2f(md.x - M);
-    D += w * md.y;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      acc[k].x += w * v[k].x;
-      acc[k].y += w * v[k].y;
-      acc[k].z += w * v[k].z;
-      acc[k].w += w * v[k].w;
-    }
-  };
-#pragma unroll 4
-  for (int i = 0; i < n_pre; ++i) add(pre + i * pre_seg, pitch);
-  bool any = n_pre > 0;
-#pragma unroll 2
-  for (int gg = glo; gg <= ghi; ++gg) {
-    if (!sp.nonempty(gg)) continue;
-    add(own + gg * kOwnSeg, kGqa);
-    any = true;
-  }
-  const float inv = any ? 1.f / D : 0.f;  // no entries at all: output 0, LSE -inf
-  const int row = h * kGqa + r;
-  __nv_bfloat16* orow = p.out + int64_t(b) * p.out_stride_tok + int64_t(row) * p.out_stride_head;
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    *reinterpret_cast<uint2*>(orow + (cg + 8 * k) * 4) =
-        make_uint2(pack_bf16x2(acc[k].x * inv, acc[k].y * inv), pack_bf16x2(acc[k].z * inv, acc[k].w * inv));
-  if (p.lse != nullptr && cg == 0) p.lse[int64_t(b) * kNumQoHeads + row] = any ? M + log2f(D) : -INFINITY;
-}
-
-// With SharedDecodeParams the token axis holds the requests' own entries behind a shared prefix: every segment
-// leaves a partial state, and the last warp to finish a request joins them with the prefix's states, once the
-// prefix kernel, beside which this one may run, has ended.
-template <class Cfg, class Params>
-__global__ void __launch_bounds__(Cfg::THREADS, 1) tiered_decode_kernel(const __grid_constant__ Params p) {
-  constexpr bool kShared = std::is_same<Params, SharedDecodeParams>::value;
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::THREADS, 1) tiered_decode_kernel(const __grid_constant__ TieredDecodeParams p) {
   constexpr int NS = Cfg::NS, TILE = Cfg::TILE, CONS = Cfg::CONSUMERS;
   constexpr int IC = Cfg::IDX_CHUNK, IB = Cfg::IDX_BUFS;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -339,14 +250,6 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1) tiered_decode_kernel(const __
   constexpr int kDeferredMerges = 4;
   int deferred[kDeferredMerges];  // requests this warp merges once its range is done
   int n_deferred = 0;
-  auto merge = [&](int b, int glo, int ghi) {
-    if constexpr (kShared) {
-      asm volatile("griddepcontrol.wait;" ::: "memory");  // the prefix kernel's states
-      merge_shared_prefix(p, sp, b, h, glo, ghi, lane);
-    } else {
-      merge_request_heads(p, sp, b, h, glo, ghi, lane);
-    }
-  };
 
   auto load_q = [&](int b) {
     if (gi < kGqa) {
@@ -445,22 +348,10 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1) tiered_decode_kernel(const __
       split_bf16x2(pr[0], pr[1], pa0, pl0);
       split_bf16x2(pr[2], pr[3], pa2, pl2);
       // ---- O += P V
-      // the entries of this lane's V words (2 ci, 2 ci + 1 and the same + 8) that exist
-      const int last = rows - 2 * ci;
-      const uint32_t keep0 = last > 1 ? ~0u : last == 1 ? 0xffffu : 0u;
-      const uint32_t keep1 = last > 9 ? ~0u : last == 9 ? 0xffffu : 0u;
 #pragma unroll
       for (int dp = 0; dp < 8; ++dp) {
         uint32_t b0, b1, b2, b3;
         ldmatrix_x4_trans(b0, b1, b2, b3, sV + ((mi & 1) * 8 + rr) * Cfg::PITCH + (dp * 16 + (mi >> 1) * 8) * 2);
-        if constexpr (kShared) {
-          if (rows < TILE) {  // rows past the end hold an earlier tile's values: 0 x inf is not 0
-            b0 &= keep0;
-            b1 &= keep1;
-            b2 &= keep0;
-            b3 &= keep1;
-          }
-        }
         mma_bf16_16816(o[2 * dp], pa0, pl0, pa2, pl2, b0, b1);
         mma_bf16_16816(o[2 * dp + 1], pa0, pl0, pa2, pl2, b2, b3);
       }
@@ -474,16 +365,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1) tiered_decode_kernel(const __
       int64_t start, end;
       sp.range(p.indptr, cur_b, start, end);
       const bool whole = start >= lo && end <= hi;  // the request lies inside this CTA's range
-      if constexpr (kShared) {
-        if (gi < kGqa) {
-          float* dst = p.partial + ((int64_t(g + cur_b) * kNumKvHeads + h) * kOwnState + gi) * 4;
-#pragma unroll
-          for (int nt = 0; nt < 16; ++nt)
-            *reinterpret_cast<float2*>(dst + (nt * 2 + (ci >> 1)) * (kGqa * 4) + (ci & 1) * 2) =
-                make_float2(o[nt][0] + o[nt][2], o[nt][1] + o[nt][3]);
-          if (ci == 0) *reinterpret_cast<float2*>(dst + (kStateGroups - 1) * (kGqa * 4)) = make_float2(m_run, d_row);
-        }
-      } else if (gi < kGqa) {
+      if (gi < kGqa) {
         if (whole) {
           // ---- normalise and write the output directly
           const float inv = 1.f / d_row;
@@ -504,15 +386,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1) tiered_decode_kernel(const __
         }
       }
       reset_state();
-      if (kShared && whole) {
-        if (n_deferred < kDeferredMerges) {
-          deferred[n_deferred++] = cur_b;
-        } else {
-          __threadfence();
-          __syncwarp();
-          merge(cur_b, g, g);
-        }
-      } else if (!whole) {
+      if (!whole) {
         // the last of the request's CTAs to arrive for this kv head merges the partial states
         __syncwarp();
         const int glo = sp.owner(start), ghi = sp.owner(end - 1);
@@ -533,7 +407,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1) tiered_decode_kernel(const __
             deferred[n_deferred++] = cur_b;
           } else {
             __threadfence();
-            merge(cur_b, glo, ghi);
+            merge_request_heads(p, sp, cur_b, h, glo, ghi, lane);
           }
         }
       }
@@ -542,20 +416,10 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1) tiered_decode_kernel(const __
 
   // ---- the merges this warp deferred (it was the last of their CTAs to arrive)
   if (n_deferred > 0) __threadfence();
-  if (kShared) __syncwarp();
   for (int i = 0; i < n_deferred; ++i) {
     int64_t start, end;
     sp.range(p.indptr, deferred[i], start, end);
-    merge(deferred[i], sp.owner(start), sp.owner(end - 1));
-  }
-
-  if constexpr (kShared) {  // requests with no entries of their own, spread over the CTAs
-    for (int b = g; b < p.batch; b += G) {
-      int64_t start, end;
-      sp.range(p.indptr, b, start, end);
-      if (end <= start) merge(b, 0, -1);
-    }
-    return;
+    merge_request_heads(p, sp, deferred[i], h, sp.owner(start), sp.owner(end - 1), lane);
   }
 
   // ---- requests with no KV entries: output 0, LSE -inf, written by the CTA that owns their
@@ -587,32 +451,10 @@ int decode_default_grid_g(int device) {
 cudaError_t launch_tiered_decode(const TieredDecodeParams& p, cudaStream_t stream) {
   using Cfg = DecodeCfg;
   static std::atomic<uint64_t> configured{0};
-  if (cudaError_t e = set_max_dynamic_smem_once(tiered_decode_kernel<Cfg, TieredDecodeParams>, Cfg::SMEM_BYTES,
-                                                configured))
+  if (cudaError_t e = set_max_dynamic_smem_once(tiered_decode_kernel<Cfg>, Cfg::SMEM_BYTES, configured))
     return e;
   tiered_decode_kernel<Cfg><<<p.grid_g, Cfg::THREADS, Cfg::SMEM_BYTES, stream>>>(p);
   return cudaGetLastError();
-}
-
-// Started while the prefix kernel in front of it still runs (programmatic stream serialization): its CTAs take
-// the SMs that the prefix leaves, and wait for its end only before they join states.
-cudaError_t launch_shared_decode(const SharedDecodeParams& p, cudaStream_t stream) {
-  using Cfg = DecodeCfg;
-  static std::atomic<uint64_t> configured{0};
-  if (cudaError_t e = set_max_dynamic_smem_once(tiered_decode_kernel<Cfg, SharedDecodeParams>, Cfg::SMEM_BYTES,
-                                                configured))
-    return e;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(unsigned(p.grid_g));
-  config.blockDim = dim3(Cfg::THREADS);
-  config.dynamicSmemBytes = Cfg::SMEM_BYTES;
-  config.stream = stream;
-  config.attrs = &attr;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, tiered_decode_kernel<Cfg, SharedDecodeParams>, p);
 }
 
 }  // namespace dual

@@ -1,30 +1,37 @@
-// Attention of many requests' single query tokens over a prefix that they share (the prefix part of a
-// shared-prefix decode), on the 5th-generation tensor cores.
+// Decode of a batch whose requests share prefixes: every prefix is attended once for all of its requests on the
+// 5th-generation tensor cores, each request's own entries on their own, and the partial softmax states are joined.
 //
-// Mathematics.  For request b of a group and its prefix's entries j: partial softmax states
-//   m = max_j x_bj,  d = sum_j 2^(x_bj - m),  O = sum_j 2^(x_bj - m) V_j,   x_bj = scale log2(e) q_b K_j,
-// one per segment of the prefix; tiered_decode_kernel joins them with the state of the request's own entries.
+// Mathematics.  For request b, its prefix's entries and its own, with x_bj = scale log2(e) q_b K_j: the states
+//   m = max_j x_bj,  d = sum_j 2^(x_bj - m),  O = sum_j 2^(x_bj - m) V_j
+// of disjoint parts of the entries join to one: m = max m_i, d = sum 2^(m_i - m) d_i, O likewise; the output is
+// O / d, the base-2 log-sum-exp m + log2 d.  All states are held in 32 bits.
 // Read by each request alone, a prefix of P entries costs a batch of B requests 4096 B P bytes; here the
 // group's requests are the rows of one matrix product, and every K / V row is read once per block of 64
 // requests.  Up to about 64 requests the bytes bound it (64 requests x 16,384 operations per entry of 4,096
 // bytes are 256 operations per byte, the ratio of the card's measured rates is 251), above that the
-// tensor cores and the exponentials.
+// tensor cores and the exponentials; the requests' own entries are bound by bytes.
 //
-// Work: a job is (block of up to 64 requests, kv head); the plan lays the jobs' kv tiles end to end and cuts
-// them into one equal range per CTA (one CTA per SM), so a CTA works on one or a few segments, each a part of
-// one job, and a long prefix of a small batch still fills the GPU.
+// Work.  Prefixes: a job is (block of up to 64 requests, kv head); the plan lays the jobs' kv tiles end to end
+// and cuts them into one equal range per CTA (one CTA per SM), so a CTA works on one or a few segments, each a
+// part of one job, and a long prefix of a small batch still fills the GPU.  Own entries: the flattened token
+// axis is cut into one range per CTA as in tiered_decode_kernel.  Every CTA does both, the prefix first.  (With
+// half of the CTAs in the other order, so that one part's products would overlap the other's loads, 256 requests
+// over 16,384 entries and up to 600 of their own took 201 us instead of 158.)  shared_join_kernel joins the states; it is launched beside the first and waits for its end.
 //
-// One CTA, warp-specialised; two streams of 128 rows x 128 entries alternate on the tensor core, one in
+// Prefix phase, warp-specialised; two streams of 128 rows x 128 entries alternate on the tensor core, one in
 // softmax while the other is in its products:
 //   * a block of 33 to 64 requests is two query tiles (32 requests x 4 heads of the group = 128 rows each),
 //     and both streams see every kv tile;
 //   * a block of up to 32 requests is one query tile, and the streams take the kv tiles in turn (even, odd);
 //     their two states are joined in the epilogue.  With one stream alone the chain product -> softmax ->
 //     product, not the memory, would set the pace.
-// Loader warps gather K and V tiles (128 entries x 256 B of the kv head) into a ring of swizzled tiles, the
-// MMA warp issues O_s += P_s V and S_s = Q K^T (P in tensor memory over its own S), a softmax warpgroup per
-// stream turns S into P with one thread per row; the running maximum moves only when it grows by more than
-// 2^8.  All waits are bounded; one that runs out records DUAL_STATUS_WAIT_TIMEOUT and every role unwinds.
+// Loader warps gather K and V tiles (128 entries x 256 B of the kv head) into a ring of swizzled tiles in the
+// order in which the products take them, the MMA warp issues O_s += P_s V and S_s = Q K^T (P in tensor memory
+// over its own S), a softmax warpgroup per stream turns S into P with one thread per row; the running maximum
+// moves only when it grows by more than 2^8.
+// Own phase: one warp issues a bulk copy per row and plane (2 KiB, all kv heads), eight warps, one per kv head,
+// multiply 16 entries at a time with the 4 query heads of the group as the rows of warp-level products.
+// All waits are bounded; one that runs out records DUAL_STATUS_WAIT_TIMEOUT and every role unwinds.
 #include <algorithm>
 #include <type_traits>
 #include <vector>
@@ -40,7 +47,8 @@ constexpr int kTileTok = 32;                   // requests per query tile
 constexpr int kRows = kTileTok * kGqa;         // 128 rows of the products
 constexpr int kStreams = 2;
 constexpr int kBN = 128;                       // kv entries per kv tile
-constexpr int kSlots = 5;                      // ring slots, each one K or one V tile
+constexpr int kSlots = 5;                      // ring slots, each one K or one V tile; one more where the second
+                                               // query tile's room is free
 constexpr int kLoadWarps = 4;
 constexpr int kLoadThreads = kLoadWarps * 32;
 constexpr int kWarpEntries = kBN / kLoadWarps;  // entries of a tile that one loader warp gathers: a lane each
@@ -57,7 +65,13 @@ constexpr int kOffSlot = kStreams * kQBytes;
 constexpr int kOffExchange = kOffSlot + kSlots * kSlotBytes;  // (m, d) of each stream's rows
 constexpr int kOffPeer = kOffExchange + kStreams * kRows * 8;  // supplier banks' pointers
 constexpr int kOffBar = kOffPeer + 2 * kMaxPeers * 8;
-constexpr int kNumBars = 2 * kSlots + 4 * kStreams + 4;
+// own phase, in the room of the query tiles and the ring
+using Own = DecodeCfg;
+static_assert(Own::CONSUMERS == kSoftmaxWarps, "a consumer warp per kv head");
+constexpr int kOffIds = Own::NS * Own::STAGE_BYTES;  // page ids
+static_assert(kOffIds + Own::IDX_BUFS * Own::IDX_CHUNK * 4 <= kOffExchange, "own phase's shared memory");
+
+constexpr int kNumBars = 2 * (kSlots + 1) + 4 * kStreams + 4 + 2 * Own::NS + Own::IDX_BUFS;
 constexpr int kSmemBytes = kOffBar + kNumBars * 8 + 16;
 static_assert(kSmemBytes <= 232448, "shared memory budget");
 
@@ -74,75 +88,157 @@ __device__ __forceinline__ void cp_async_mbar_arrive_noinc(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
+// D = A B + D where only rows 0..7 of the 16 x 16 A hold anything: the other rows' registers are zeros.
+__device__ __forceinline__ void mma_bf16_8x8x16(float* d, uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
+  float unused0, unused1;
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%9,%9};"
+      : "+f"(d[0]), "+f"(d[1]), "=f"(unused0), "=f"(unused1)
+      : "r"(a0), "r"(0u), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 struct Segment {
   int tok0, ntok, head, kv0, kv1, flags;
-  int64_t state;  // float offset
+  int64_t state;  // 16-byte units
   bool single;    // one query tile, the streams take kv tiles in turn
   __device__ __forceinline__ int tiles() const { return (kv1 - kv0 + kBN - 1) / kBN; }
   // kv tiles of stream s, and the i-th of them
   __device__ __forceinline__ int tiles_of(int s) const { return single ? (tiles() + 1 - s) / 2 : tiles(); }
   __device__ __forceinline__ int tile(int s, int i) const { return single ? 2 * i + s : i; }
+  // The ring holds tiles in the order in which the products take them.  Both streams on every tile:
+  // K0 V0 K1 V1 ...; tiles in turn: K0 K1 V0 K2 V1 K3 V2 ... (stream s needs K(t + 2) right after V(t)).
+  __device__ __forceinline__ int fill_of_k(int t) const { return !single ? 2 * t : t == 0 ? 0 : 2 * t - 1; }
+  __device__ __forceinline__ int fill_of_v(int t) const { return !single || t == tiles() - 1 ? 2 * t + 1 : 2 * t + 2; }
 };
 
-// Segment `i` of the plan; false (and a status bit) where it does not fit this call's tensors.
-__device__ __forceinline__ bool load_segment(const SharedPrefixParams& p, const PlanView& plan, int i, Segment& g) {
-  const int4* w = reinterpret_cast<const int4*>(plan.words + plan.segment_at() + int64_t(i) * kSegmentWords);
-  const int4 a = __ldg(w), b = __ldg(w + 1);
+// Segment `i` of CTA `cta` (of `count`; the second is at `second` among the segments); false (and a status bit)
+// where it does not fit this call's tensors.
+__device__ __forceinline__ bool load_segment(const SharedPrefixParams& p, int second, int i, Segment& g) {
+  const int32_t* at = i == 0 ? p.plan + kPlanHeader + int64_t(blockIdx.x) * kCtaWords + 4
+                             : p.plan + kPlanHeader + int64_t(p.ctas) * kCtaWords + int64_t(second + i - 1) * kSegmentWords;
+  const int4 a = __ldg(reinterpret_cast<const int4*>(at)), b = __ldg(reinterpret_cast<const int4*>(at) + 1);
   g.tok0 = a.x;
   g.ntok = a.y;
   g.head = a.z;
   g.kv0 = a.w;
   g.kv1 = b.x;
-  g.state = int64_t(uint32_t(b.y)) * 4;
+  g.state = uint32_t(b.y);
   g.flags = b.z;
   g.single = g.ntok <= kTileTok;
   const bool ok = g.tok0 >= 0 && g.ntok > 0 && g.ntok <= kBlockRequests && g.tok0 <= p.batch - g.ntok && g.head >= 0 &&
-                  g.head < kNumKvHeads && g.kv0 >= 0 && g.kv0 < g.kv1 && g.kv1 <= p.num_indices &&
-                  g.state / 4 + int64_t(kStateGroups) * kGqa * g.ntok <= p.state_size;
+                  g.head < kNumKvHeads && g.kv0 >= 0 && g.kv0 < g.kv1 && g.kv1 <= p.num_prefix &&
+                  (g.single || !(g.flags & kSegDeep)) &&
+                  g.state + int64_t(kStateGroups) * kGqa * g.ntok <= p.state_size;
   if (!ok && threadIdx.x == 0) atomicOr(p.status, kStatusBadLength);
   return ok;
 }
 
-__global__ void __launch_bounds__(kThreads, 1) shared_prefix_kernel(const __grid_constant__ SharedPrefixParams p) {
+// The requests' own entries: the flattened token axis [0, T) over G CTAs, CTA g owning [g T / G, (g + 1) T / G)
+// (positions are int32, as in indptr).  A CTA has a tile at least, so that a request is not cut into more states
+// than it has tiles.
+struct OwnSplit {
+  int T, G;
+  bool bad;
+  __device__ __forceinline__ OwnSplit(const SharedPrefixParams& p) {
+    T = __ldg(p.indptr + p.batch);
+    bad = T > p.num_indices || T < 0;
+    if (bad) T = T < 0 ? 0 : int(p.num_indices);
+    G = max(1, min(p.ctas, T / Own::TILE));
+  }
+  __device__ __forceinline__ int begin(int g) const { return g >= G ? T : int((int64_t(g) * T) / G); }
+  __device__ __forceinline__ int owner(int x) const { return int((int64_t(x + 1) * G - 1) / T); }
+};
+
+// Walks the tiles of a CTA's range [lo, hi); tiles never straddle a request.  init() is executed by whole warps.
+struct OwnIter {
+  int t0, seg_hi, hi, b;
+  __device__ __forceinline__ void init(int lo, int hi_, const int32_t* indptr, int batch, int lane) {
+    hi = seg_hi = hi_;
+    t0 = lo;
+    b = 0;
+    if (lo >= hi) return;
+    int l = 0, r = batch;  // the first request whose end exceeds lo is in [l, r): 32 probes at a time
+    while (r - l > 1) {
+      const int step = (r - l + 31) / 32;
+      const int at = min(l + (lane + 1) * step, r) - 1;
+      const unsigned past = __ballot_sync(0xffffffffu, __ldg(indptr + at + 1) > lo);
+      const int f = past ? __ffs(past) - 1 : 31;
+      l = min(l + f * step, r - 1);
+      r = min(l + step, r);
+    }
+    b = l;
+    seg_hi = min(hi, __ldg(indptr + b + 1));
+    if (seg_hi <= t0) t0 = hi;  // only reachable with a non-monotone indptr
+  }
+  __device__ __forceinline__ bool valid() const { return t0 < hi; }
+  __device__ __forceinline__ int rows() const { return min(Own::TILE, seg_hi - t0); }
+  __device__ __forceinline__ bool last_in_segment() const { return seg_hi - t0 <= Own::TILE; }
+  __device__ __forceinline__ void next(const int32_t* indptr, int batch) {
+    t0 += rows();
+    if (t0 >= seg_hi && t0 < hi) {
+      do {
+        if (b + 1 >= batch) {  // only reachable with a non-monotone indptr: stop, never read past it
+          t0 = hi;
+          return;
+        }
+        ++b;
+        seg_hi = min(hi, __ldg(indptr + b + 1));
+      } while (seg_hi <= t0);
+    }
+  }
+};
+
+__global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid_constant__ SharedPrefixParams p) {
   // No static shared memory, so the dynamic part starts on the 1024-byte boundary that the swizzled tiles
   // need (there is no room to align it here); checked below.
   extern __shared__ __align__(1024) unsigned char smem[];
   float2* exchange = reinterpret_cast<float2*>(smem + kOffExchange);  // [stream][row]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
-  uint64_t* slot_full = bars;                    // [kSlots] count kLoadThreads
-  uint64_t* slot_empty = bars + kSlots;          // [kSlots] count 1 (tcgen05.commit)
-  uint64_t* s_full = bars + 2 * kSlots;          // [2]      count 1 (tcgen05.commit)
-  uint64_t* p_part = s_full + kStreams;          // [2 x 2]  count 128: P of entries 32..127, then 0..31
-  uint64_t* o_done = p_part + 2 * kStreams;      // [2]      count 1 (tcgen05.commit, a segment's last PV)
-  uint64_t* q_full = o_done + kStreams;          // count kLoadThreads
-  uint64_t* q_empty = q_full + 1;                // count 1 (tcgen05.commit, a segment's last QK)
-  uint64_t* x_full = q_full + 2;                 // count kSoftmaxThreads: (m, d) of both streams written
-  uint64_t* x_done = q_full + 3;                 // count kSoftmaxThreads: both streams' O read
+  uint64_t* slot_full = bars;                       // [6]      count kLoadThreads
+  uint64_t* slot_empty = slot_full + kSlots + 1;    // [6]      count 1 (tcgen05.commit)
+  uint64_t* s_full = slot_empty + kSlots + 1;       // [2]      count 1 (tcgen05.commit)
+  uint64_t* p_part = s_full + kStreams;             // [2 x 2]  count 128: P of entries 32..127, then 0..31
+  uint64_t* o_done = p_part + 2 * kStreams;         // [2]      count 1 (tcgen05.commit, a segment's last PV)
+  uint64_t* q_full = o_done + kStreams;             // count kLoadThreads
+  uint64_t* q_empty = q_full + 1;                   // count 1 (tcgen05.commit, a segment's last QK)
+  uint64_t* x_full = q_full + 2;                    // count kSoftmaxThreads: (m, d) of both streams written
+  uint64_t* x_done = q_full + 3;                    // count kSoftmaxThreads: both streams' O read
+  uint64_t* own_full = q_full + 4;                  // [NS]     count 1 + bytes
+  uint64_t* own_empty = own_full + Own::NS;         // [NS]     count 8
+  uint64_t* ids_full = own_empty + Own::NS;         // [3]      count 32
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + kNumBars);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars) + 1;
+  const char** const s_peer = reinterpret_cast<const char**>(smem + kOffPeer);  // K, then V; indexed at run time
 
-  // the kernel behind this one in the stream reads other memory until it waits for this one's end
+  // the kernel behind this one in the stream waits for this one's end before it reads its states
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // everything that the first loads depend on, in one round trip
+  const int4 cta_words = __ldg(reinterpret_cast<const int4*>(p.plan + kPlanHeader + int64_t(blockIdx.x) * kCtaWords));
+  const int first_flags = __ldg(p.plan + kPlanHeader + int64_t(blockIdx.x) * kCtaWords + 10);
+  const OwnSplit split(p);
   PlanView plan;
-  if (!plan.open(p.plan, p.plan_words) || plan.ctas != int(gridDim.x) || plan.requests != p.batch ||
-      (smem_addr(smem) & 1023u) != 0) {
+  bool planned = plan.open(p.plan, p.plan_words) && plan.ctas == p.ctas && plan.requests == p.batch;
+  int nseg = cta_words.x;
+  const int second = cta_words.y;
+  planned = planned && nseg >= 0 && second >= 0 && (nseg <= 1 || second <= plan.segments - (nseg - 1));
+  if ((smem_addr(smem) & 1023u) != 0) planned = false;
+  if (!planned) {
     if (tid == 0) atomicOr(p.status, kStatusBadLength);
-    return;
+    nseg = 0;
   }
-  const int seg0 = max(0, __ldg(plan.words + plan.cta_at() + blockIdx.x));
-  const int seg1 = min(plan.segments, __ldg(plan.words + plan.cta_at() + blockIdx.x + 1));
-  if (seg0 >= seg1) return;
+  if (split.bad && tid == 0) atomicOr(p.status, kStatusBadLength);
+  const int own_lo = split.begin(blockIdx.x), own_hi = split.begin(blockIdx.x + 1);
+  if (nseg == 0 && own_lo >= own_hi) return;
 
-  const char** const s_peer = reinterpret_cast<const char**>(smem + kOffPeer);  // K, then V; indexed at run time
   if (tid == 0) {
 #pragma unroll
     for (int i = 0; i < kMaxPeers; ++i) {
       s_peer[i] = p.peer_k[i];
       s_peer[kMaxPeers + i] = p.peer_v[i];
     }
-    for (int s = 0; s < kSlots; ++s) {
+    for (int s = 0; s < kSlots + 1; ++s) {
       mbar_init(slot_full + s, kLoadThreads);
       mbar_init(slot_empty + s, 1);
     }
@@ -156,6 +252,11 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_kernel(const __grid
     mbar_init(q_empty, 1);
     mbar_init(x_full, kSoftmaxThreads);
     mbar_init(x_done, kSoftmaxThreads);
+    for (int s = 0; s < Own::NS; ++s) {
+      mbar_init(own_full + s, 1);
+      mbar_init(own_empty + s, Own::CONSUMERS);
+    }
+    for (int s = 0; s < Own::IDX_BUFS; ++s) mbar_init(ids_full + s, 32);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -177,79 +278,91 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_kernel(const __grid
   // every lane of a warp goes on, or none: the loops below hold warp-collective instructions
   auto wait_warp = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
 
-  if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
-    // ================================================================ loaders
-    const int lt = tid - kSoftmaxThreads;  // 0 .. kLoadThreads - 1
-    const int lw = lt >> 5;
-    const int half = lane >> 4, chunk = lane & 15;
-    const char* const k_local = p.k_local;
-    const char* const v_local = p.v_local;
-    const int64_t local_stride = p.local_stride, peer_stride = p.peer_stride, peer_slots = p.peer_slots;
-    const uint32_t capacity = static_cast<uint32_t>(p.local_capacity);
-    const uint32_t np = static_cast<uint32_t>(max(p.num_peers, 0));
-    unsigned* const status = p.status;
-    // page id -> row pointers of both planes (page 0 of the local pool for a bad remote id, which is
-    // recorded in the status word)
-    auto resolve = [&](int32_t page_id, const char*& kp, const char*& vp) {
-      const uint32_t page = static_cast<uint32_t>(page_id);
-      if (page <= capacity) {
-        kp = k_local + int64_t(page) * local_stride;
-        vp = v_local + int64_t(page) * local_stride;
+  const int slots = kSlots + (nseg > 0 && (first_flags & kSegDeep) ? 1 : 0);
+  auto slot_of = [&](int u) { return slots == kSlots ? u % kSlots : u % (kSlots + 1); };
+  auto turn_of = [&](int u) { return slots == kSlots ? u / kSlots : u / (kSlots + 1); };
+  auto slot_offset = [&](int s) { return s == kSlots ? kQBytes : kOffSlot + s * kSlotBytes; };
+  // page id -> row pointers of both planes (page 0 of the local pool for a bad remote id, which is
+  // recorded in the status word)
+  auto resolve = [&](int32_t page_id, const char*& kp, const char*& vp) {
+    const uint32_t page = static_cast<uint32_t>(page_id), capacity = static_cast<uint32_t>(p.local_capacity);
+    if (page <= capacity) {
+      kp = p.k_local + int64_t(page) * p.local_stride;
+      vp = p.v_local + int64_t(page) * p.local_stride;
+    } else {
+      const uint32_t np = static_cast<uint32_t>(p.num_peers), gid = page - capacity - 1u;
+      const uint32_t bank = np > 0 ? gid % np : 0u;
+      const uint32_t phys = np > 0 ? gid / np : 0u;
+      if (np == 0 || int64_t(phys) >= p.peer_slots) {
+        atomicOr(p.status, kStatusBadRemoteSlot);
+        kp = p.k_local;
+        vp = p.v_local;
       } else {
-        const uint32_t gid = page - capacity - 1u;
-        const uint32_t bank = np > 0 ? gid % np : 0u;
-        const uint32_t phys = np > 0 ? gid / np : 0u;
-        if (np == 0 || int64_t(phys) >= peer_slots) {
-          atomicOr(status, kStatusBadRemoteSlot);
-          kp = k_local;
-          vp = v_local;
-        } else {
-          kp = s_peer[bank] + int64_t(phys) * peer_stride;
-          vp = s_peer[kMaxPeers + bank] + int64_t(phys) * peer_stride;
-        }
+        kp = s_peer[bank] + int64_t(phys) * p.peer_stride;
+        vp = s_peer[kMaxPeers + bank] + int64_t(phys) * p.peer_stride;
       }
-    };
-    auto shfl_ptr = [](const char* ptr, int src_lane) {
-      const unsigned long long v = reinterpret_cast<unsigned long long>(ptr);
-      const uint32_t lo = __shfl_sync(0xffffffffu, static_cast<uint32_t>(v), src_lane);
-      const uint32_t hi = __shfl_sync(0xffffffffu, static_cast<uint32_t>(v >> 32), src_lane);
-      return reinterpret_cast<const char*>((static_cast<unsigned long long>(hi) << 32) | lo);
-    };
-    int u = 0, nq = 0;  // ring fills and query loads so far
-    bool ok = true;
-    for (int i = seg0; i < seg1 && ok; ++i) {
-      Segment g;
-      if (!load_segment(p, plan, i, g)) continue;
-      const int64_t off = g.head * 256 + chunk * 16;
-      const int ntiles = g.tiles(), len = g.kv1 - g.kv0;
-      const int32_t* const indices = p.indices + g.kv0;
-      auto page_of = [&](int j) -> int32_t {  // page id of this lane's entry of tile j (0 past the end)
-        const int pos = j * kBN + kWarpEntries * lw + lane;
-        return pos < len ? __ldg(indices + pos) : 0;
-      };
-      const char *kr, *vr;  // row pointers of this lane's entry, one tile ahead of use
-      resolve(page_of(0), kr, vr);
-      int32_t next = ntiles > 1 ? page_of(1) : 0;
-      for (int j = 0; j < ntiles && ok; ++j) {
-        const int32_t after = j + 2 < ntiles ? page_of(j + 2) : 0;  // lands while this tile is issued
-#pragma unroll 1
-        for (int plane = 0; plane < 2; ++plane) {  // K then V of tile j
-          const int s = u % kSlots, f = u / kSlots;
-          if (f > 0 && !wait_warp(slot_empty + s, uint32_t(f - 1) & 1u)) {
+    }
+  };
+  auto shfl_ptr = [](const char* ptr, int src_lane) {
+    const unsigned long long v = reinterpret_cast<unsigned long long>(ptr);
+    const uint32_t lo = __shfl_sync(0xffffffffu, static_cast<uint32_t>(v), src_lane);
+    const uint32_t hi = __shfl_sync(0xffffffffu, static_cast<uint32_t>(v >> 32), src_lane);
+    return reinterpret_cast<const char*>((static_cast<unsigned long long>(hi) << 32) | lo);
+  };
+
+  // ---- prefix phase
+  auto prefix_phase = [&]() {
+    if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
+      // ============================================================== loaders
+      const int lt = tid - kSoftmaxThreads;  // 0 .. kLoadThreads - 1
+      const int lw = lt >> 5;
+      const int half = lane >> 4, chunk = lane & 15;
+      int nq = 0, u0 = 0;  // query loads, ring fills of the segments before
+      bool ok = true;
+      for (int i = 0; i < nseg && ok; ++i) {
+        Segment g;
+        if (!load_segment(p, second, i, g)) continue;
+        const int64_t off = g.head * 256 + chunk * 16;
+        const int ntiles = g.tiles(), len = g.kv1 - g.kv0;
+        const int32_t* const indices = p.prefix + g.kv0;
+        auto page_of = [&](int j) -> int32_t {  // page id of this lane's entry of tile j (0 past the end)
+          const int pos = j * kBN + kWarpEntries * lw + lane;
+          return pos < len ? __ldg(indices + pos) : 0;
+        };
+        // row pointers of this lane's entry: K and V of the newest tile, V of the one before
+        const char *kr = nullptr, *vr = nullptr, *vr_before = nullptr;
+        int32_t next = page_of(0), after = ntiles > 1 ? page_of(1) : 0;
+        const int fills = 2 * ntiles;
+        for (int f = 0; f < fills; ++f) {
+          // which tile this is (the inverse of fill_of_k / fill_of_v)
+          const bool is_k = g.single ? f == 0 || ((f & 1) && f < fills - 1) : !(f & 1);
+          const int t = !g.single ? f >> 1 : f == fills - 1 ? ntiles - 1 : is_k ? (f + 1) >> 1 : (f >> 1) - 1;
+          const char* row;
+          if (is_k) {
+            vr_before = vr;
+            resolve(next, kr, vr);
+            next = after;
+            after = t + 2 < ntiles ? page_of(t + 2) : 0;  // lands while this tile is issued
+            row = kr;
+          } else {
+            row = g.single && f < fills - 1 ? vr_before : vr;
+          }
+          const int u = u0 + f;
+          const int s = slot_of(u), turn = turn_of(u);
+          if (turn > 0 && !wait_warp(slot_empty + s, uint32_t(turn - 1) & 1u)) {
             ok = false;
             break;
           }
-          unsigned char* dst_tile = smem + kOffSlot + s * kSlotBytes;
+          unsigned char* dst_tile = smem + slot_offset(s);
+          const int valid = len - t * kBN - kWarpEntries * lw;
 #pragma unroll 8
           for (int e = 0; e < kWarpEntries / 2; ++e) {
             const int rr = 2 * e + half;
-            const int row = kWarpEntries * lw + rr;
-            const char* src = shfl_ptr(plane == 0 ? kr : vr, rr);
-            cp_async_16_zfill(dst_tile + tc::sw128_offset<kBN>(row, chunk), src + off, j * kBN + row < len);
+            const char* src = shfl_ptr(row, rr);
+            cp_async_16_zfill(dst_tile + tc::sw128_offset<kBN>(kWarpEntries * lw + rr, chunk), src + off, rr < valid);
           }
           cp_async_mbar_arrive_noinc(slot_full + s);
-          ++u;
-          if (j == 0 && plane == 0) {
+          if (f == 0) {
             // the query tiles, behind the first K tile so that it is on its way while the last
             // segment's products still read the old ones; rows past the block are zero
             if (nq > 0 && !wait_warp(q_empty, uint32_t(nq - 1) & 1u)) {
@@ -260,311 +373,472 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_kernel(const __grid
             const int rows = g.single ? kRows : kStreams * kRows;
             for (int r = lt >> 4; r < rows; r += kLoadThreads / 16) {
               const int tok = r / kGqa;
-              const bool valid = tok < g.ntok;
-              const __nv_bfloat16* src = p.q + int64_t(g.tok0 + (valid ? tok : 0)) * p.q_stride_tok +
+              const bool there = tok < g.ntok;
+              const __nv_bfloat16* src = p.q + int64_t(g.tok0 + (there ? tok : 0)) * p.q_stride_tok +
                                          int64_t(g.head * kGqa + r % kGqa) * p.q_stride_head + chunk * 8;
-              cp_async_16_zfill(smem + (r / kRows) * kQBytes + tc::sw128_offset<kRows>(r % kRows, chunk), src, valid);
+              cp_async_16_zfill(smem + (r / kRows) * kQBytes + tc::sw128_offset<kRows>(r % kRows, chunk), src, there);
             }
             cp_async_mbar_arrive_noinc(q_full);
           }
         }
-        if (j + 1 < ntiles) resolve(next, kr, vr);
-        next = after;
+        u0 += fills;
       }
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp == kMmaWarp) {
-    // ================================================================ MMA issue
-    // The whole warp runs the loop in uniform control flow, one elected lane issues.
-    const bool leader = tc::elect_one();
-    constexpr uint32_t kIdescQK = tc::idesc_bf16_f32(128, kBN, 0, 0);
-    constexpr uint32_t kIdescPV = tc::idesc_bf16_f32(128, 128, 0, 1);
-    const uint32_t q_base = smem_addr(smem);
-    const uint32_t slot_base = smem_addr(smem + kOffSlot);
-    auto slot_addr = [&](int u) { return slot_base + uint32_t(u % kSlots) * kSlotBytes; };
-    auto slot_wait = [&](int u) { return wait_warp(slot_full + u % kSlots, uint32_t(u / kSlots) & 1u); };
-    auto slot_free = [&](int u) {
-      if (leader) tc::commit(slot_empty + u % kSlots);
-    };
-    int u0 = 0, nseg = 0;        // ring fills of the segments before, segments before
-    int np0 = 0, np1 = 0;        // P tiles taken from each stream
-    bool ok = true;
-    for (int i = seg0; i < seg1 && ok; ++i) {
-      Segment g;
-      if (!load_segment(p, plan, i, g)) continue;
-      const int ntiles = g.tiles(), steps = g.tiles_of(0);
-      const bool residual = (g.flags & kSegResidual) != 0;
-      // O_s (+)= P_s V(tile), in the two parts in which the softmax hands P over (entries 32..127, 0..31)
-      auto issue_pv = [&](int s, int t, bool first) -> bool {
-        int& np = s == 0 ? np0 : np1;
-        const uint32_t v_base = slot_addr(u0 + 2 * t + 1);
-        const uint32_t tP = tmem + s * kBN, tO = tmem + kColO + s * 128;
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          if (!wait_warp(p_part + 2 * s + part, uint32_t(np) & 1u)) return false;
-          tc::fence_after_sync();
-#pragma unroll
-          for (int k = 0; k < (part == 0 ? 6 : 2); ++k) {
-            const int kb = part == 0 ? 2 + k : k;
-            const uint64_t vdesc = tc::smem_desc_sw128(v_base + kb * 2048, kBN * 128, 1024);
-            const uint32_t ph = tP + 32 * (kb >> 1) + 8 * (kb & 1);
-            if (leader) {
-              tc::mma_bf16_ts(tO, ph, vdesc, kIdescPV, (!first || part > 0 || k > 0) ? 1u : 0u);
-              if (residual) tc::mma_bf16_ts(tO, ph + 16, vdesc, kIdescPV, 1u);
-            }
-          }
-        }
-        ++np;
-        return true;
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp == kMmaWarp) {
+      // ============================================================== MMA issue
+      // The whole warp runs the loop in uniform control flow, one elected lane issues.
+      const bool leader = tc::elect_one();
+      constexpr uint32_t kIdescQK = tc::idesc_bf16_f32(128, kBN, 0, 0);
+      constexpr uint32_t kIdescPV = tc::idesc_bf16_f32(128, 128, 0, 1);
+      const uint32_t base = smem_addr(smem);
+      int u0 = 0, nq = 0;    // ring fills of the segments before, query tiles so far
+      int np0 = 0, np1 = 0;  // P tiles taken from each stream
+      auto slot_wait = [&](int f) { return wait_warp(slot_full + slot_of(u0 + f), uint32_t(turn_of(u0 + f)) & 1u); };
+      auto slot_free = [&](int f) {
+        if (leader) tc::commit(slot_empty + slot_of(u0 + f));
       };
-      ok = wait_warp(q_full, uint32_t(nseg) & 1u);
-      for (int j = 0; j < steps && ok; ++j) {
-        for (int s = 0; s < kStreams && ok; ++s) {
-          const int t = g.tile(s, j);
-          if (t >= ntiles) break;  // the odd stream has one tile less
-          // K(t) landed, and with it every earlier tile: a loader thread arrives on a slot only once all of
-          // its earlier copies have landed
-          if (s == 0 || g.single) {
-            ok = slot_wait(u0 + 2 * t);
-            if (!ok) break;
-            fence_proxy_async_smem();  // cp.async writes -> tensor core reads
+      bool ok = true;
+      for (int i = 0; i < nseg && ok; ++i) {
+        Segment g;
+        if (!load_segment(p, second, i, g)) continue;
+        const int ntiles = g.tiles(), steps = g.tiles_of(0);
+        const bool residual = (g.flags & kSegResidual) != 0;
+        // O_s (+)= P_s V(t), in the two parts in which the softmax hands P over (entries 32..127, 0..31)
+        auto issue_pv = [&](int s, int t, bool first) -> bool {
+          int& np = s == 0 ? np0 : np1;
+          const uint32_t v_base = base + slot_offset(slot_of(u0 + g.fill_of_v(t)));
+          const uint32_t tP = tmem + s * kBN, tO = tmem + kColO + s * 128;
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            if (!wait_warp(p_part + 2 * s + part, uint32_t(np) & 1u)) return false;
             tc::fence_after_sync();
-          }
-          if (j > 0) {
-            ok = issue_pv(s, g.tile(s, j - 1), j == 1);
-            if (!ok) break;
-            if (g.single) slot_free(u0 + 2 * g.tile(s, j - 1) + 1);
-          }
-          const uint32_t qb = q_base + (g.single ? 0 : s) * kQBytes, kb0 = slot_addr(u0 + 2 * t);
 #pragma unroll
-          for (int kb = 0; kb < 8; ++kb) {
-            const uint32_t off_q = (kb >> 2) * (kRows * 128) + (kb & 3) * 32;
-            const uint32_t off_k = (kb >> 2) * (kBN * 128) + (kb & 3) * 32;
-            if (leader)
-              tc::mma_bf16(tmem + s * kBN, tc::smem_desc_sw128(qb + off_q, 16, 1024),
-                           tc::smem_desc_sw128(kb0 + off_k, 16, 1024), kIdescQK, kb > 0);
-          }
-          if (leader) tc::commit(s_full + s);  // S_s written, the PV before it done
-          if (g.single) slot_free(u0 + 2 * t);
-        }
-        if (ok && !g.single) {
-          slot_free(u0 + 2 * j);
-          if (j > 0) slot_free(u0 + 2 * j - 1);
-        }
-      }
-      if (!ok) break;
-      if (leader) tc::commit(q_empty);
-      ok = slot_wait(u0 + 2 * ntiles - 1);
-      if (ok) fence_proxy_async_smem();
-      for (int s = 0; s < kStreams && ok; ++s) {
-        const int n = g.tiles_of(s);
-        if (n == 0) continue;
-        ok = issue_pv(s, g.tile(s, n - 1), n == 1);
-        if (!ok) break;
-        if (leader) tc::commit(o_done + s);
-        if (g.single || s == 1) slot_free(u0 + 2 * g.tile(s, n - 1) + 1);
-      }
-      u0 += 2 * ntiles;
-      ++nseg;
-    }
-  } else {
-    // ================================================================ softmax, a warpgroup per stream
-    const int s = warp / 4;
-    const int r = tid - s * kRows;  // row = tensor memory lane
-    const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + s * kBN + lane_base;
-    const uint32_t tO = tmem + kColO + lane_base;  // O of stream 0; stream 1's is 128 columns on
-    const float scale = p.scale_log2;
-    int ns = 0, no0 = 0, no1 = 0, nx = 0;  // S tiles of this stream, last PVs of each, exchanges so far
-    bool ok = true;
-    for (int i = seg0; i < seg1 && ok; ++i) {
-      Segment g;
-      if (!load_segment(p, plan, i, g)) continue;
-      const int n = g.tiles_of(s), len = g.kv1 - g.kv0;
-      const bool residual = (g.flags & kSegResidual) != 0;
-      float m_used = -INFINITY, d_sum = 0.f;  // m_used in the scaled (log2) domain
-      for (int j = 0; j < n; ++j) {
-        if (!wait_warp(s_full + s, uint32_t(ns) & 1u)) {
-          ok = false;
-          break;
-        }
-        ++ns;
-        tc::fence_after_sync();
-        const int vis = len - g.tile(s, j) * kBN;  // entries of this tile, 128 or more where it is whole
-        const bool needs_mask = vis < kBN;
-        // scores in two halves of 64 columns: maximum over both, the second half stays live for the
-        // exponentials and the first is read again afterwards
-        float x[64];
-        auto load_half = [&](int c0) {
-          tc::ld32(tS + c0, x);
-          tc::ld32(tS + c0 + 32, x + 32);
-          tc::wait_ld();
-          if (needs_mask) {
-#pragma unroll
-            for (int c = 0; c < 64; ++c) x[c] = c0 + c < vis ? x[c] : -INFINITY;
-          }
-        };
-        auto half_max = [&]() {
-          float m4[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-          for (int c = 4; c < 60; c += 8) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) m4[e] = fmax3(m4[e], x[c + e], x[c + 4 + e]);
-          }
-          return fmax3(fmax3(m4[0], m4[1], x[60]), fmax3(m4[2], m4[3], x[61]), fmaxf(x[62], x[63]));
-        };
-        load_half(0);
-        float tmax = half_max();
-        load_half(64);
-        tmax = fmaxf(tmax, half_max()) * scale;
-        float alpha = 1.f;
-        bool rescale = false;
-        if (tmax > m_used + kRescaleThreshold) {
-          alpha = fast_exp2(m_used - tmax);  // 0 on the first tile
-          m_used = tmax;
-          rescale = true;
-        }
-        // O_s is quiescent here: the PV before this S is done, the next one waits for this P
-        if (j > 0 && __any_sync(0xffffffffu, rescale)) {
-          const float a = rescale ? alpha : 1.f;
-#pragma unroll 1
-          for (int c0 = 0; c0 < 128; c0 += 32) {
-            float o[32];
-            tc::ld32(tO + s * 128 + c0, o);
-            tc::wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] *= a;
-            tc::st32(tO + s * 128 + c0, o);
-          }
-        }
-        const uint64_t scale2 = f2_pack(scale, scale), neg_m2 = f2_pack(-m_used, -m_used);
-        uint64_t rs2[4] = {0, 0, 0, 0};  // packed partial row sums, four independent chains
-        auto emit_p = [&](const float* xc, int col, auto lo_tag) {
-          constexpr bool kLo = decltype(lo_tag)::value;
-#pragma unroll
-          for (int sub = 0; sub < 2; ++sub) {  // 16 entries: 8 high words, 8 residual words
-            uint32_t hi[8], lo[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              float t0, t1;
-              f2_unpack(f2_fma(f2_pack(xc[16 * sub + 2 * e], xc[16 * sub + 2 * e + 1]), scale2, neg_m2), t0, t1);
-              const float p0 = fast_exp2(t0), p1 = fast_exp2(t1);
-              const uint64_t pp = f2_pack(p0, p1);
-              rs2[e & 3] = f2_add(rs2[e & 3], pp);
-              hi[e] = pack_bf16x2(p0, p1);
-              if (kLo) {
-                const uint64_t hh = f2_pack(__uint_as_float(hi[e] << 16), __uint_as_float(hi[e] & 0xffff0000u));
-                float l0, l1;
-                f2_unpack(f2_sub(pp, hh), l0, l1);
-                lo[e] = pack_bf16x2(l0, l1);
+            for (int k = 0; k < (part == 0 ? 6 : 2); ++k) {
+              const int kb = part == 0 ? 2 + k : k;
+              const uint64_t vdesc = tc::smem_desc_sw128(v_base + kb * 2048, kBN * 128, 1024);
+              const uint32_t ph = tP + 32 * (kb >> 1) + 8 * (kb & 1);
+              if (leader) {
+                tc::mma_bf16_ts(tO, ph, vdesc, kIdescPV, (!first || part > 0 || k > 0) ? 1u : 0u);
+                if (residual) tc::mma_bf16_ts(tO, ph + 16, vdesc, kIdescPV, 1u);
               }
             }
-            tc::st8u(tS + col + 8 * sub, hi);
-            if (kLo) tc::st8u(tS + col + 16 + 8 * sub, lo);
           }
+          ++np;
+          return true;
         };
-        auto emit = [&](const float* xc, int col) {
-          if (residual)
-            emit_p(xc, col, std::true_type{});
-          else
-            emit_p(xc, col, std::false_type{});
-        };
-        auto mask32 = [&](float* xc, int col) {
-          if (needs_mask) {
+        ok = wait_warp(q_full, uint32_t(nq) & 1u);
+        for (int j = 0; j < steps && ok; ++j) {
+          for (int s = 0; s < kStreams && ok; ++s) {
+            const int t = g.tile(s, j);
+            if (t >= ntiles) break;  // the odd stream has one tile less
+            // K(t) landed, and with it every earlier tile of the ring: a loader thread arrives on a slot only
+            // once all of its earlier copies have landed
+            if (s == 0 || g.single) {
+              ok = slot_wait(g.fill_of_k(t));
+              if (!ok) break;
+              fence_proxy_async_smem();  // cp.async writes -> tensor core reads
+              tc::fence_after_sync();
+            }
+            if (j > 0) {
+              ok = issue_pv(s, g.tile(s, j - 1), j == 1);
+              if (!ok) break;
+              if (g.single || s == 1) slot_free(g.fill_of_v(g.tile(s, j - 1)));
+            }
+            const uint32_t qb = base + (g.single ? 0 : s) * kQBytes, kb0 = base + slot_offset(slot_of(u0 + g.fill_of_k(t)));
 #pragma unroll
-            for (int c = 0; c < 32; ++c) xc[c] = col + c < vis ? xc[c] : -INFINITY;
+            for (int kb = 0; kb < 8; ++kb) {
+              const uint32_t off_q = (kb >> 2) * (kRows * 128) + (kb & 3) * 32;
+              const uint32_t off_k = (kb >> 2) * (kBN * 128) + (kb & 3) * 32;
+              if (leader)
+                tc::mma_bf16(tmem + s * kBN, tc::smem_desc_sw128(qb + off_q, 16, 1024),
+                             tc::smem_desc_sw128(kb0 + off_k, 16, 1024), kIdescQK, kb > 0);
+            }
+            if (leader) tc::commit(s_full + s);  // S_s written, the PV before it done
+            if (g.single || s == 1) slot_free(g.fill_of_k(t));
           }
-        };
-        // x holds entries 64..127; entries 0..63 are read again into each half of x once it is consumed
-        emit(x, 64);
-        tc::ld32(tS, x);
-        emit(x + 32, 96);
-        tc::ld32(tS + 32, x + 32);
-        tc::wait_ld();
-        mask32(x + 32, 32);
-        emit(x + 32, 32);
-        tc::wait_st();
-        tc::fence_before_sync();
-        mbar_arrive(p_part + 2 * s);
-        mask32(x, 0);
-        emit(x, 0);
-        float r0, r1, r2, r3;
-        f2_unpack(f2_add(rs2[0], rs2[1]), r0, r1);
-        f2_unpack(f2_add(rs2[2], rs2[3]), r2, r3);
-        d_sum = d_sum * alpha + ((r0 + r1) + (r2 + r3));
-        tc::wait_st();
-        tc::fence_before_sync();
-        mbar_arrive(p_part + 2 * s + 1);
+        }
+        if (!ok) break;
+        if (leader) tc::commit(q_empty);
+        ok = slot_wait(2 * ntiles - 1);
+        if (ok) fence_proxy_async_smem();
+        for (int s = 0; s < kStreams && ok; ++s) {
+          const int n = g.tiles_of(s);
+          if (n == 0) continue;
+          ok = issue_pv(s, g.tile(s, n - 1), n == 1);
+          if (!ok) break;
+          if (leader) tc::commit(o_done + s);
+          if (g.single || s == 1) slot_free(g.fill_of_v(g.tile(s, n - 1)));
+        }
+        u0 += 2 * ntiles;
+        ++nq;
       }
-      if (!ok) break;
-      // ---- the segment's state: unnormalised O, m, d
-      const int rows = kGqa * g.ntok;
-      float4* const dst = reinterpret_cast<float4*>(p.states + g.state);
-      const int n1 = g.tiles_of(1);
-      if (g.single || s == 0) ok = wait_warp(o_done, uint32_t(no0) & 1u);
-      if (ok && n1 > 0 && (g.single || s == 1)) ok = wait_warp(o_done + 1, uint32_t(no1) & 1u);
-      if (!ok) break;
-      ++no0;
-      no1 += n1 > 0;
-      tc::fence_after_sync();
-      if (!g.single) {
-        const int row = s * kRows + r;
-#pragma unroll 1
-        for (int c0 = 0; c0 < 128; c0 += 32) {
-          float o[32];
-          tc::ld32(tO + s * 128 + c0, o);
-          tc::wait_ld();
-          if (row < rows) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              dst[((c0 + e) >> 2) * rows + row] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+    } else {
+      // ============================================================== softmax, a warpgroup per stream
+      const int s = warp / 4;
+      const int r = tid - s * kRows;  // row = tensor memory lane
+      const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
+      const uint32_t tS = tmem + s * kBN + lane_base;
+      const uint32_t tO = tmem + kColO + lane_base;  // O of stream 0; stream 1's is 128 columns on
+      const float scale = p.scale_log2;
+      int ns = 0, no0 = 0, no1 = 0, nx = 0;  // S tiles of this stream, last PVs of each, exchanges so far
+      bool ok = true;
+      for (int i = 0; i < nseg && ok; ++i) {
+        Segment g;
+        if (!load_segment(p, second, i, g)) continue;
+        const int n = g.tiles_of(s), len = g.kv1 - g.kv0;
+        const bool residual = (g.flags & kSegResidual) != 0;
+        float m_used = -INFINITY, d_sum = 0.f;  // m_used in the scaled (log2) domain
+        for (int j = 0; j < n; ++j) {
+          if (!wait_warp(s_full + s, uint32_t(ns) & 1u)) {
+            ok = false;
+            break;
           }
-        }
-        if (row < rows) dst[(kStateGroups - 1) * rows + row] = make_float4(m_used, d_sum, 0.f, 0.f);
-      } else {
-        // both streams hold states of the same rows: each group joins half of the columns
-        exchange[s * kRows + r] = make_float2(m_used, d_sum);
-        mbar_arrive(x_full);
-        if (!wait_warp(x_full, uint32_t(nx) & 1u)) {
-          ok = false;
-          break;
-        }
-        const float2 a = exchange[r], b = exchange[kRows + r];
-        const float m = fmaxf(a.x, b.x);
-        const float wa = fast_exp2(a.x - m), wb = n1 > 0 ? fast_exp2(b.x - m) : 0.f;
-#pragma unroll 1
-        for (int c0 = 64 * s; c0 < 64 * s + 64; c0 += 32) {
-          float o[32];
-          tc::ld32(tO + c0, o);
-          tc::wait_ld();
+          ++ns;
+          tc::fence_after_sync();
+          const int vis = len - g.tile(s, j) * kBN;  // entries of this tile, 128 or more where it is whole
+          const bool needs_mask = vis < kBN;
+          // scores in two halves of 64 columns: maximum over both, the second half stays live for the
+          // exponentials and the first is read again afterwards
+          float x[64];
+          auto load_half = [&](int c0) {
+            tc::ld32(tS + c0, x);
+            tc::ld32(tS + c0 + 32, x + 32);
+            tc::wait_ld();
+            if (needs_mask) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] *= wa;
-          if (n1 > 0) {
-            float o1[32];
-            tc::ld32(tO + 128 + c0, o1);
+              for (int c = 0; c < 64; ++c) x[c] = c0 + c < vis ? x[c] : -INFINITY;
+            }
+          };
+          auto half_max = [&]() {
+            float m4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+            for (int c = 4; c < 60; c += 8) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) m4[e] = fmax3(m4[e], x[c + e], x[c + 4 + e]);
+            }
+            return fmax3(fmax3(m4[0], m4[1], x[60]), fmax3(m4[2], m4[3], x[61]), fmaxf(x[62], x[63]));
+          };
+          load_half(0);
+          float tmax = half_max();
+          load_half(64);
+          tmax = fmaxf(tmax, half_max()) * scale;
+          float alpha = 1.f;
+          bool rescale = false;
+          if (tmax > m_used + kRescaleThreshold) {
+            alpha = fast_exp2(m_used - tmax);  // 0 on the first tile
+            m_used = tmax;
+            rescale = true;
+          }
+          // O_s is quiescent here: the PV before this S is done, the next one waits for this P
+          if (j > 0 && __any_sync(0xffffffffu, rescale)) {
+            const float a = rescale ? alpha : 1.f;
+#pragma unroll 1
+            for (int c0 = 0; c0 < 128; c0 += 32) {
+              float o[32];
+              tc::ld32(tO + s * 128 + c0, o);
+              tc::wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] *= a;
+              tc::st32(tO + s * 128 + c0, o);
+            }
+          }
+          const uint64_t scale2 = f2_pack(scale, scale), neg_m2 = f2_pack(-m_used, -m_used);
+          uint64_t rs2[4] = {0, 0, 0, 0};  // packed partial row sums, four independent chains
+          auto emit_p = [&](const float* xc, int col, auto lo_tag) {
+            constexpr bool kLo = decltype(lo_tag)::value;
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub) {  // 16 entries: 8 high words, 8 residual words
+              uint32_t hi[8], lo[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                float t0, t1;
+                f2_unpack(f2_fma(f2_pack(xc[16 * sub + 2 * e], xc[16 * sub + 2 * e + 1]), scale2, neg_m2), t0, t1);
+                const float p0 = fast_exp2(t0), p1 = fast_exp2(t1);
+                const uint64_t pp = f2_pack(p0, p1);
+                rs2[e & 3] = f2_add(rs2[e & 3], pp);
+                hi[e] = pack_bf16x2(p0, p1);
+                if (kLo) {
+                  const uint64_t hh = f2_pack(__uint_as_float(hi[e] << 16), __uint_as_float(hi[e] & 0xffff0000u));
+                  float l0, l1;
+                  f2_unpack(f2_sub(pp, hh), l0, l1);
+                  lo[e] = pack_bf16x2(l0, l1);
+                }
+              }
+              tc::st8u(tS + col + 8 * sub, hi);
+              if (kLo) tc::st8u(tS + col + 16 + 8 * sub, lo);
+            }
+          };
+          auto emit = [&](const float* xc, int col) {
+            if (residual)
+              emit_p(xc, col, std::true_type{});
+            else
+              emit_p(xc, col, std::false_type{});
+          };
+          auto mask32 = [&](float* xc, int col) {
+            if (needs_mask) {
+#pragma unroll
+              for (int c = 0; c < 32; ++c) xc[c] = col + c < vis ? xc[c] : -INFINITY;
+            }
+          };
+          // x holds entries 64..127; entries 0..63 are read again into each half of x once it is consumed
+          emit(x, 64);
+          tc::ld32(tS, x);
+          emit(x + 32, 96);
+          tc::ld32(tS + 32, x + 32);
+          tc::wait_ld();
+          mask32(x + 32, 32);
+          emit(x + 32, 32);
+          tc::wait_st();
+          tc::fence_before_sync();
+          mbar_arrive(p_part + 2 * s);
+          mask32(x, 0);
+          emit(x, 0);
+          float r0, r1, r2, r3;
+          f2_unpack(f2_add(rs2[0], rs2[1]), r0, r1);
+          f2_unpack(f2_add(rs2[2], rs2[3]), r2, r3);
+          d_sum = d_sum * alpha + ((r0 + r1) + (r2 + r3));
+          tc::wait_st();
+          tc::fence_before_sync();
+          mbar_arrive(p_part + 2 * s + 1);
+        }
+        if (!ok) break;
+        // ---- the segment's state: unnormalised O, m, d
+        const int rows = kGqa * g.ntok;
+        float4* const dst = reinterpret_cast<float4*>(p.states) + g.state;
+        const int n1 = g.tiles_of(1);
+        if (g.single || s == 0) ok = wait_warp(o_done, uint32_t(no0) & 1u);
+        if (ok && n1 > 0 && (g.single || s == 1)) ok = wait_warp(o_done + 1, uint32_t(no1) & 1u);
+        if (!ok) break;
+        ++no0;
+        no1 += n1 > 0;
+        tc::fence_after_sync();
+        if (!g.single) {
+          const int row = s * kRows + r;
+#pragma unroll 1
+          for (int c0 = 0; c0 < 128; c0 += 16) {
+            float o[16];
+            tc::ld16(tO + s * 128 + c0, o);
+            tc::wait_ld();
+            if (row < rows) {
+#pragma unroll
+              for (int e = 0; e < 16; e += 4)
+                dst[((c0 + e) >> 2) * rows + row] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+          }
+          if (row < rows) dst[(kStateGroups - 1) * rows + row] = make_float4(m_used, d_sum, 0.f, 0.f);
+        } else {
+          // both streams hold states of the same rows: each group joins half of the columns
+          exchange[s * kRows + r] = make_float2(m_used, d_sum);
+          mbar_arrive(x_full);
+          if (!wait_warp(x_full, uint32_t(nx) & 1u)) {
+            ok = false;
+            break;
+          }
+          const float2 a = exchange[r], b = exchange[kRows + r];
+          const float m = fmaxf(a.x, b.x);
+          const float wa = fast_exp2(a.x - m), wb = n1 > 0 ? fast_exp2(b.x - m) : 0.f;
+#pragma unroll 1
+          for (int c0 = 64 * s; c0 < 64 * s + 64; c0 += 16) {
+            float o[16], o1[16];
+            tc::ld16(tO + c0, o);
+            tc::ld16(tO + 128 + c0, o1);  // not written by any product where n1 = 0
             tc::wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] += wb * o1[e];
-          }
-          if (r < rows) {
+            for (int e = 0; e < 16; ++e) o[e] = wa * o[e] + (n1 > 0 ? wb * o1[e] : 0.f);
+            if (r < rows) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              dst[((c0 + e) >> 2) * rows + r] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+              for (int e = 0; e < 16; e += 4)
+                dst[((c0 + e) >> 2) * rows + r] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
           }
+          if (s == 0 && r < rows)
+            dst[(kStateGroups - 1) * rows + r] = make_float4(m, wa * a.y + (n1 > 0 ? wb * b.y : 0.f), 0.f, 0.f);
+          tc::fence_before_sync();
+          mbar_arrive(x_done);
+          if (!wait_warp(x_done, uint32_t(nx) & 1u)) {
+            ok = false;
+            break;
+          }
+          ++nx;
         }
-        if (s == 0 && r < rows)
-          dst[(kStateGroups - 1) * rows + r] = make_float4(m, wa * a.y + (n1 > 0 ? wb * b.y : 0.f), 0.f, 0.f);
-        tc::fence_before_sync();
-        mbar_arrive(x_done);
-        if (!wait_warp(x_done, uint32_t(nx) & 1u)) {
-          ok = false;
-          break;
-        }
-        ++nx;
       }
     }
-  }
+  };
+  // ---- own phase
+  auto own_phase = [&]() {
+    if (warp == kSoftmaxWarps) {
+      // ============================================================== row copies
+      OwnIter it;
+      it.init(own_lo, own_hi, p.indptr, p.batch, lane);
+      int32_t* const sidx = reinterpret_cast<int32_t*>(smem + kOffIds);
+      constexpr int IC = Own::IDX_CHUNK, IB = Own::IDX_BUFS;
+      const int r = lane & 15;
+      const bool is_v = lane >= 16;
+      const uint64_t policy = l2_policy_evict_first();
+      const int nchunks = (own_hi - own_lo + IC - 1) / IC;
+      int issued = 0, ready = -1;
+      auto issue_chunk = [&](int c) {
+        const int buf = c % IB;
+        const int first = own_lo + c * IC;
+        for (int i = lane; i < IC; i += 32)
+          if (first + i < own_hi) cp_async_4(sidx + buf * IC + i, p.indices + first + i);
+        cp_async_mbar_arrive_noinc(ids_full + buf);
+      };
+      while (issued < nchunks && issued < IB) issue_chunk(issued++);
+      int n_issued = 0;
+      for (; it.valid(); it.next(p.indptr, p.batch), ++n_issued) {
+        const int rows = it.rows();
+        const int c_first = (it.t0 - own_lo) / IC, c_last = (it.t0 + rows - 1 - own_lo) / IC;
+        while (issued < nchunks && issued <= c_first + IB - 1) issue_chunk(issued++);
+        bool ok = !*abort_flag;
+        while (ok && ready < c_last) {
+          ++ready;
+          ok = wait(ids_full + (ready % IB), uint32_t(ready / IB) & 1u);
+        }
+        const int stage = n_issued % Own::NS, fill = n_issued / Own::NS;
+        if (ok && fill > 0) ok = wait(own_empty + stage, uint32_t(fill - 1) & 1u);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (lane == 0) mbar_arrive_expect_tx(own_full + stage, uint32_t(rows) * 2u * Own::ROW_BYTES);
+        __syncwarp();
+        if (r < rows) {
+          const int off = it.t0 + r - own_lo;
+          const char *kr, *vr;
+          resolve(sidx[(off / IC) % IB * IC + off % IC], kr, vr);
+          bulk_g2s_hint(smem + stage * Own::STAGE_BYTES + (is_v ? Own::PLANE_BYTES : 0) + r * Own::PITCH, is_v ? vr : kr,
+                        Own::ROW_BYTES, own_full + stage, policy);
+        }
+      }
+      // never leave the phase with copies still landing in shared memory
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      for (int k = 0; k < min(n_issued, Own::NS); ++k) {
+        const int n = n_issued - 1 - k;
+        if (!mbar_wait_bounded(own_full + n % Own::NS, uint32_t(n / Own::NS) & 1u)) {
+          *abort_flag = 1;
+          atomicOr(p.status, kStatusWaitTimeout);
+          break;
+        }
+      }
+    } else if (warp < kSoftmaxWarps) {
+      // ============================================================== products, a warp per kv head
+      const int h = warp;
+      const int gi = lane >> 2, ci = lane & 3;
+      OwnIter it;
+      it.init(own_lo, own_hi, p.indptr, p.batch, lane);
+      // Rows 0..3 of a product are the 4 query heads, rows 4..7 the same heads again: P's high part goes into
+      // the first, its bf16 residual into the second, and their outputs are added when a state is written.
+      uint32_t qa[8][2];
+      float o[16][2];
+      float m_run = -INFINITY, d_run = 0.f;
+#pragma unroll
+      for (int nt = 0; nt < 16; ++nt) o[nt][0] = o[nt][1] = 0.f;
+      int cur_b = -1, n_seen = 0;
+      for (; it.valid(); it.next(p.indptr, p.batch), ++n_seen) {
+        if (it.b != cur_b) {
+          cur_b = it.b;
+          const __nv_bfloat16* qrow =
+              p.q + int64_t(cur_b) * p.q_stride_tok + int64_t(h * kGqa + (gi & 3)) * p.q_stride_head;
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            qa[ks][0] = *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 2 * ci);
+            qa[ks][1] = *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 8 + 2 * ci);
+          }
+        }
+        const int stage = n_seen % Own::NS;
+        const int rows = it.rows();
+        if (!wait_warp(own_full + stage, uint32_t(n_seen / Own::NS) & 1u)) break;
+        const unsigned char* sK = smem + stage * Own::STAGE_BYTES + h * kHeadDim * 2;
+        const unsigned char* sV = sK + Own::PLANE_BYTES;
+        const int mi = lane >> 3, rr = lane & 7;
+        // ---- S = Q K^T  (rows: 4 q heads, columns: 16 entries)
+        float s[2][2];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          s[nt][0] = s[nt][1] = 0.f;
+#pragma unroll
+          for (int kp = 0; kp < 4; ++kp) {
+            uint32_t b0, b1, b2, b3;
+            ldmatrix_x4(b0, b1, b2, b3, sK + (nt * 8 + rr) * Own::PITCH + (kp * 32 + mi * 8) * 2);
+            mma_bf16_8x8x16(s[nt], qa[2 * kp][0], qa[2 * kp][1], b0, b1);
+            mma_bf16_8x8x16(s[nt], qa[2 * kp + 1][0], qa[2 * kp + 1][1], b2, b3);
+          }
+        }
+        // ---- online softmax in the log2 domain; the running maximum moves only by more than 2^8
+        float x[4] = {s[0][0] * p.scale_log2, s[0][1] * p.scale_log2, s[1][0] * p.scale_log2, s[1][1] * p.scale_log2};
+        const int left = rows - 2 * ci;  // this lane's entries are 2 ci, 2 ci + 1 and the same + 8
+        if (left < 1) x[0] = -INFINITY;
+        if (left < 2) x[1] = -INFINITY;
+        if (left < 9) x[2] = -INFINITY;
+        if (left < 10) x[3] = -INFINITY;
+        float tmax = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 1));
+        tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 2));
+        float alpha = 1.f;
+        if (tmax > m_run + kRescaleThreshold) {
+          alpha = fast_exp2(m_run - tmax);  // 0 on a request's first tile
+          m_run = tmax;
+        }
+        float pr[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pr[e] = fast_exp2(x[e] - m_run);
+        d_run = d_run * alpha + (pr[0] + pr[1]) + (pr[2] + pr[3]);
+        if (__any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+          for (int nt = 0; nt < 16; ++nt) {
+            o[nt][0] *= alpha;
+            o[nt][1] *= alpha;
+          }
+        }
+        uint32_t hi0, hi2, lo0, lo2;
+        split_bf16x2(pr[0], pr[1], hi0, lo0);
+        split_bf16x2(pr[2], pr[3], hi2, lo2);
+        const uint32_t pa0 = gi < kGqa ? hi0 : lo0, pa2 = gi < kGqa ? hi2 : lo2;
+        // ---- O += P V; rows past the end hold whatever was there, and 0 x inf is not 0
+        const uint32_t keep0 = left > 1 ? ~0u : left == 1 ? 0xffffu : 0u;
+        const uint32_t keep1 = left > 9 ? ~0u : left == 9 ? 0xffffu : 0u;
+#pragma unroll
+        for (int dp = 0; dp < 8; ++dp) {
+          uint32_t b0, b1, b2, b3;
+          ldmatrix_x4_trans(b0, b1, b2, b3, sV + ((mi & 1) * 8 + rr) * Own::PITCH + (dp * 16 + (mi >> 1) * 8) * 2);
+          if (rows < Own::TILE) {
+            b0 &= keep0;
+            b1 &= keep1;
+            b2 &= keep0;
+            b3 &= keep1;
+          }
+          mma_bf16_8x8x16(o[2 * dp], pa0, pa2, b0, b1);
+          mma_bf16_8x8x16(o[2 * dp + 1], pa0, pa2, b2, b3);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(own_empty + stage);
+        if (it.last_in_segment()) {
+          float d_row = d_run;
+          d_row += __shfl_xor_sync(0xffffffffu, d_row, 1);
+          d_row += __shfl_xor_sync(0xffffffffu, d_row, 2);
+          float* dst = p.own + ((int64_t(blockIdx.x + cur_b) * kNumKvHeads + h) * kOwnState + (gi & 3)) * 4;
+#pragma unroll
+          for (int nt = 0; nt < 16; ++nt) {
+            o[nt][0] += __shfl_xor_sync(0xffffffffu, o[nt][0], 16);
+            o[nt][1] += __shfl_xor_sync(0xffffffffu, o[nt][1], 16);
+            if (gi < kGqa)
+              *reinterpret_cast<float2*>(dst + (nt * 2 + (ci >> 1)) * (kGqa * 4) + (ci & 1) * 2) =
+                  make_float2(o[nt][0], o[nt][1]);
+            o[nt][0] = o[nt][1] = 0.f;
+          }
+          if (gi < kGqa && ci == 0)
+            *reinterpret_cast<float2*>(dst + (kStateGroups - 1) * (kGqa * 4)) = make_float2(m_run, d_row);
+          m_run = -INFINITY;
+          d_run = 0.f;
+        }
+      }
+    }
+  };
+  if (nseg > 0) prefix_phase();
+  // the own phase has its tiles where the prefix phase had its own, written and read by other units
+  fence_proxy_async_smem();
   tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  if (own_lo < own_hi && !*abort_flag) own_phase();
   __syncthreads();
   if (warp == kMmaWarp) {
     if (*abort_flag) {
@@ -576,6 +850,108 @@ __global__ void __launch_bounds__(kThreads, 1) shared_prefix_kernel(const __grid
     }
     tc::dealloc(tmem, kTmemCols);
   }
+}
+
+constexpr int kJoinThreads = 128;  // one block per (request, kv head)
+constexpr int kJoinStates = 8;     // states at a time
+
+__device__ __forceinline__ float4 ld_state(const float4* p) {  // past L1, behind the wait (volatile)
+  float4 v;
+  asm volatile("ld.global.cg.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+
+// Joins the states of a request and kv head: of its own entries (one per CTA that holds a part of them) and of its
+// group's prefix (one per segment).  Thread = (row lane % 4, column group), so that four lanes read 64 consecutive
+// bytes; eight states at a time, each lane with (m, d) of one of them and a column group of all, the weights
+// passed by shuffle.  Bound by latency: what is known before the states is read before the wait, and the code is
+// short (unrolled over all states with two rows per warp it took 1 us per state, most of it instruction fetch).
+__global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_constant__ SharedPrefixParams p) {
+  const int lane = threadIdx.x & 31;
+  const int b = blockIdx.x / kNumKvHeads, h = blockIdx.x % kNumKvHeads;
+  const int r = lane & 3, cg = threadIdx.x >> 2;  // row, column group
+  const float4* pre = reinterpret_cast<const float4*>(p.states);
+  const float4* own = reinterpret_cast<const float4*>(p.own) + h * kOwnState + r;
+  constexpr int64_t kOwnSeg = int64_t(kNumKvHeads) * kOwnState;
+  int n_pre = 0, n_own = 0;
+  int64_t pitch = 0;
+  const int own_first = __ldg(p.indptr + b), own_last = __ldg(p.indptr + b + 1);
+  const OwnSplit split(p);
+  PlanView plan;
+  bool ok = plan.open(p.plan, p.plan_words) && plan.ctas == p.ctas && plan.requests == p.batch;
+  if (ok) {
+    const int2 req = __ldg(reinterpret_cast<const int2*>(plan.words + plan.request_at()) + b);
+    if (req.x >= 0) {
+      ok = req.x < plan.blocks;
+      const int4 job = ok ? __ldg(reinterpret_cast<const int4*>(plan.words + plan.job_at()) + req.x * kNumKvHeads + h)
+                          : make_int4(0, 0, 0, 0);
+      const int64_t off = uint32_t(job.x);
+      pitch = int64_t(kGqa) * job.z;
+      ok = ok && job.y >= 0 && job.z > 0 && job.z <= kBlockRequests && req.y >= 0 && req.y < job.z &&
+           off + int64_t(job.y) * kStateGroups * pitch <= p.state_size;
+      if (ok) {
+        pre += off + kGqa * req.y + r;
+        n_pre = job.y;
+      }
+    }
+  }
+  if (!ok && threadIdx.x == 0) atomicOr(p.status, kStatusBadLength);
+  const int start = max(0, min(own_first, split.T)), end = max(start, min(own_last, split.T));
+  if (end > start) {
+    const int first = split.owner(start);
+    n_own = split.owner(end - 1) - first + 1;
+    own += (first + int64_t(b)) * kOwnSeg;
+  }
+  const int64_t pre_seg = kStateGroups * pitch;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // states 0 .. n_pre - 1 are the prefix's, the others the request's own; past the last one the last again
+  const int n = n_pre + n_own;
+  auto load = [&](int i, int group) {
+    i = min(i, n - 1);
+    return ld_state(i < n_pre ? pre + i * pre_seg + group * pitch : own + (i - n_pre) * kOwnSeg + group * kGqa);
+  };
+  float M = -INFINITY, D = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += kJoinStates) {
+    const int mine = i0 + (lane >> 2);
+    float4 md = load(mine, kStateGroups - 1);
+    float4 v[kJoinStates];
+#pragma unroll
+    for (int e = 0; e < kJoinStates; ++e) v[e] = load(i0 + e, cg);
+    if (mine >= n) md.x = -INFINITY, md.y = 0.f;
+    float top = md.x;
+#pragma unroll
+    for (int d = 4; d <= 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    top = fmaxf(top, M);
+    const float w = md.x == -INFINITY ? 0.f : exp2f(md.x - top);
+    const float before = M == -INFINITY ? 0.f : exp2f(M - top);
+    M = top;
+    float part = w * md.y;
+#pragma unroll
+    for (int d = 4; d <= 16; d <<= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
+    D = D * before + part;
+    acc.x *= before;
+    acc.y *= before;
+    acc.z *= before;
+    acc.w *= before;
+#pragma unroll
+    for (int e = 0; e < kJoinStates; ++e) {
+      const float we = __shfl_sync(0xffffffffu, w, 4 * e + r);
+      if (i0 + e >= n) continue;
+      acc.x += we * v[e].x;
+      acc.y += we * v[e].y;
+      acc.z += we * v[e].z;
+      acc.w += we * v[e].w;
+    }
+  }
+  const float inv = n > 0 ? 1.f / D : 0.f;  // no entries at all: output 0, LSE -inf
+  const int row = h * kGqa + r;
+  __nv_bfloat16* orow = p.out + int64_t(b) * p.out_stride_tok + int64_t(row) * p.out_stride_head;
+  *reinterpret_cast<uint2*>(orow + cg * 4) =
+      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  if (p.lse != nullptr && cg == 0) p.lse[int64_t(b) * kNumQoHeads + row] = n > 0 ? M + log2f(D) : -INFINITY;
 }
 
 }  // namespace
@@ -637,27 +1013,39 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
 
   PlanView v{};
   v.ctas = ctas;
-  v.segments = int(segs.size());
+  v.segments = 0;  // beyond the CTAs' first ones
+  for (int c = 0; c < ctas; ++c) v.segments += std::max(0, cta[c + 1] - cta[c] - 1);
   v.requests = requests;
   v.blocks = int(blocks.size());
   const int64_t size = v.total();
   if (words == nullptr || max_words < size) return size;
   std::fill(words, words + size, 0);
-  std::copy(cta.begin(), cta.end(), words + v.cta_at());
   int64_t state = 0;
   std::vector<int64_t> state_of(segs.size());
-  for (size_t i = 0; i < segs.size(); ++i) {
+  auto put = [&](int32_t* w, int i, int32_t flags) {
     const Block& b = blocks[segs[i].block];
     state_of[i] = state;
-    int32_t* w = words + v.segment_at() + int64_t(i) * kSegmentWords;
     w[0] = b.tok0;
     w[1] = b.ntok;
     w[2] = segs[i].head;
     w[3] = b.kv0 + segs[i].first;
     w[4] = b.kv0 + segs[i].last;
     w[5] = int32_t(uint32_t(state));
-    w[6] = b.len < kResidualMaxEntries ? kSegResidual : 0;
+    w[6] = flags | (b.len < kResidualMaxEntries ? kSegResidual : 0);
     state += int64_t(kStateGroups) * kGqa * b.ntok;
+  };
+  int32_t* more = words + v.segment_at();
+  for (int c = 0; c < ctas; ++c) {
+    int32_t* w = words + kPlanHeader + int64_t(c) * kCtaWords;
+    w[0] = cta[c + 1] - cta[c];
+    w[1] = int32_t((more - (words + v.segment_at())) / kSegmentWords);
+    int32_t flags = kSegDeep;
+    for (int i = cta[c]; i < cta[c + 1]; ++i)
+      if (blocks[segs[i].block].ntok > kTileTok) flags = 0;
+    for (int i = cta[c]; i < cta[c + 1]; ++i) {
+      put(i == cta[c] ? w + 4 : more, i, flags);
+      if (i > cta[c]) more += kSegmentWords;
+    }
   }
   int32_t* req = words + v.request_at();
   for (int32_t i = 0; i < requests; ++i) req[2 * i] = -1;
@@ -684,11 +1072,22 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
   return size;
 }
 
-cudaError_t launch_shared_prefix(const SharedPrefixParams& p, cudaStream_t stream) {
+cudaError_t launch_shared_prefix_decode(const SharedPrefixParams& p, cudaStream_t stream) {
   static std::atomic<uint64_t> configured{0};
-  if (cudaError_t e = set_max_dynamic_smem_once(shared_prefix_kernel, kSmemBytes, configured)) return e;
-  shared_prefix_kernel<<<p.ctas, kThreads, kSmemBytes, stream>>>(p);
-  return cudaGetLastError();
+  if (cudaError_t e = set_max_dynamic_smem_once(shared_decode_kernel, kSmemBytes, configured)) return e;
+  shared_decode_kernel<<<p.ctas, kThreads, kSmemBytes, stream>>>(p);
+  if (cudaError_t e = cudaGetLastError()) return e;
+  // launched while the first kernel runs (programmatic stream serialization); it waits for its end itself
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(unsigned(p.batch) * kNumKvHeads);
+  config.blockDim = dim3(kJoinThreads);
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, shared_join_kernel, p);
 }
 
 }  // namespace dual

@@ -163,8 +163,8 @@ def shared_prefix_decode(q: torch.Tensor, k_local: torch.Tensor, v_local: torch.
                          workspace: torch.Tensor, num_ctas: int = 0) -> None:
     """One decode layer of a batch in groups that share prefixes: request b sees its group's part of
     ``prefix_indices`` and its own entries ``unified_indices[kv_indptr[b] .. kv_indptr[b + 1]]``.  ``plan``: that of
-    ``shared_prefix_plan`` on the device.  ``workspace``: ``shared_prefix_workspace_size`` bytes, its head zeroed once
-    with ``decode_workspace_reset``; the status word is its first."""
+    ``shared_prefix_plan`` on the device.  ``workspace``: ``shared_prefix_workspace_size`` bytes; its first word is the
+    status word (``status_clear`` it before the first call), the rest may hold anything."""
     dev = q.get_device()
     B = q.shape[0]
     qt, ot = q.stride(), out.stride()

@@ -201,8 +201,7 @@ class SharedPrefixDecodeWrapper:
         self._prefix = self._fill("prefix", prefix_indices, non_blocking)
         self._indptr = self._fill("indptr", indptr, non_blocking)
         self._indices = self._fill("indices", indices, non_blocking)
-        # the caller's buffer may hold anything: zero the status word and the kernels' arrival counters
-        ops.decode_workspace_reset(self._float_workspace, batch)
+        ops.status_clear(self._float_workspace)  # the caller's buffer may hold anything
         self._batch = batch
         self._sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(head_dim)
 

@@ -138,9 +138,9 @@ int dual_decode_noalloc_status(uint32_t* value_out, int device, void* stream);
  * aligned) and stays valid while the groups and the prefixes' lengths do: a decode loop that appends to
  * the requests' own lists makes it once.  num_ctas: CTAs of both launches (dual_decode_default_ctas).
  * dual_shared_prefix_workspace_size (host): bytes that a call with this plan needs; a larger workspace
- * serves smaller plans.  The workspace is the decode workspace followed by the prefixes' states: zero its
- * head once with dual_decode_workspace_reset (its counters stand behind the status word as there).
- * dual_shared_prefix_decode: two launches, the second started as the first ends.  A plan that does not
+ * serves smaller plans.  Its first 256 bytes hold the status word (clear it with dual_status_clear before
+ * the first call), the rest are partial states and may hold anything.
+ * dual_shared_prefix_decode: two launches, the second (the join of the states) started as the first ends.  A plan that does not
  * fit the call (another batch, num_ctas or index list, a workspace too small for it) records
  * DUAL_STATUS_BAD_LENGTH; the outputs are then not to be used.  Calls that share a workspace must not
  * overlap.  q, out: 16-byte aligned, element strides that are multiples of 8. */

@@ -77,7 +77,7 @@ class Case:
         ws = workspace
         if ws is None:  # partial states start as NaN: any that is read without being written shows
             ws = torch.full((ops.shared_prefix_workspace_size(plan) // 4,), float("nan"), dtype=torch.float32, device=DEV)
-        ops.decode_workspace_reset(ws, B)
+        ops.status_clear(ws)
         ops.shared_prefix_decode(q, self.k, self.v, self.C, self.bk, self.bv, self.prefix_pages, self.ii.to(DEV),
                                  self.own_pages, SCALE, plan.to(DEV), out, lse, ws, num_ctas)
         torch.cuda.synchronize()
@@ -266,12 +266,12 @@ def test_a_plan_of_another_batch_is_recorded():
     ops.shared_prefix_decode(*args, other.to(DEV), out, None, ws)
     assert int(ws.view(torch.int32)[0]) == 0x10
     longer = ops.shared_prefix_plan([0, 4], [0, 300])  # entries past the end of the index list
-    ops.decode_workspace_reset(ws, 4)
+    ops.status_clear(ws)
     big = torch.zeros(ops.shared_prefix_workspace_size(longer), dtype=torch.uint8, device=DEV)
     ops.shared_prefix_decode(*args, longer.to(DEV), out, None, big)
     assert int(big.view(torch.int32)[0]) == 0x10
     # words that are no plan: only the requests' own entries are seen
-    ops.decode_workspace_reset(ws, 4)
+    ops.status_clear(ws)
     ops.shared_prefix_decode(*args, torch.zeros(64, dtype=torch.int32, device=DEV), out, None, ws)
     assert int(ws.view(torch.int32)[0]) == 0x10
     own = Case.__new__(Case)

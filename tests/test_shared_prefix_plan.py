@@ -11,10 +11,18 @@ from dual_b200 import SharedPrefixDecodeWrapper, _lib, ops
 def read(plan):
     w = plan.tolist()
     ctas, segments, requests, blocks = w[1:5]
-    at = 8
-    cta = w[at:at + ctas + 1]
-    at = (at + ctas + 1 + 3) // 4 * 4
-    seg = [w[at + 8 * i:at + 8 * i + 8] for i in range(segments)]
+    at = 8 + 12 * ctas
+    more = [w[at + 8 * i:at + 8 * i + 8] for i in range(segments)]
+    cta, seg = [0], []
+    for c in range(ctas):  # a CTA's record holds its first segment, the others stand behind the records
+        count, second, _, _, *first = w[8 + 12 * c:20 + 12 * c]
+        mine = [first] + more[second:second + count - 1] if count else []
+        assert len(mine) == count
+        deep = all(s[1] <= 32 for s in mine)
+        assert all(bool(s[6] & 2) == deep for s in mine)
+        seg += mine
+        cta.append(len(seg))
+    assert len(more) == sum(max(0, b - a - 1) for a, b in zip(cta, cta[1:]))
     at += 8 * segments
     req = [w[at + 2 * i:at + 2 * i + 2] for i in range(requests)]
     at = (at + 2 * requests + 3) // 4 * 4
@@ -58,7 +66,7 @@ def test_segments_cover_every_prefix_once_and_states_do_not_overlap(seed):
                 assert count == len(mine)
                 for i, m in enumerate(mine):
                     assert m[2] == off + i * 33 * 4 * ntok and m[3] == local
-    assert ops.shared_prefix_workspace_size(plan) >= 16 * size + ops.decode_workspace_size(gi[-1], 1)
+    assert ops.shared_prefix_workspace_size(plan) >= 16 * size + 8 * 132 * 16 * (gi[-1] + len(cta) - 1)
 
 
 def test_work_is_even():
