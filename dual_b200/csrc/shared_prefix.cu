@@ -128,7 +128,7 @@ __device__ __forceinline__ bool load_segment(const SharedPrefixParams& p, int se
   const bool ok = g.tok0 >= 0 && g.ntok > 0 && g.ntok <= kBlockRequests && g.tok0 <= p.batch - g.ntok && g.head >= 0 &&
                   g.head < kNumKvHeads && g.kv0 >= 0 && g.kv0 < g.kv1 && g.kv1 <= p.num_prefix &&
                   (g.single || !(g.flags & kSegDeep)) &&
-                  g.state + int64_t(kStateGroups) * kGqa * g.ntok <= p.state_size;
+                  g.state + int64_t(kState) * g.ntok <= p.state_size;
   if (!ok && threadIdx.x == 0) atomicOr(p.status, kStatusBadLength);
   return ok;
 }
@@ -604,7 +604,10 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
         if (!ok) break;
         // ---- the segment's state: unnormalised O, m, d
         const int rows = kGqa * g.ntok;
-        float4* const dst = reinterpret_cast<float4*>(p.states) + g.state;
+        // of row `row`: its request's state, its place in a group
+        auto state_row = [&](int row) {
+          return reinterpret_cast<float4*>(p.states) + g.state + (row / kGqa) * kState + row % kGqa;
+        };
         const int n1 = g.tiles_of(1);
         if (g.single || s == 0) ok = wait_warp(o_done, uint32_t(no0) & 1u);
         if (ok && n1 > 0 && (g.single || s == 1)) ok = wait_warp(o_done + 1, uint32_t(no1) & 1u);
@@ -614,6 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
         tc::fence_after_sync();
         if (!g.single) {
           const int row = s * kRows + r;
+          float4* const dst = state_row(row);
 #pragma unroll 1
           for (int c0 = 0; c0 < 128; c0 += 16) {
             float o[16];
@@ -622,12 +626,13 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
             if (row < rows) {
 #pragma unroll
               for (int e = 0; e < 16; e += 4)
-                dst[((c0 + e) >> 2) * rows + row] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                dst[c0 + e] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);  // group (c0 + e) / 4 of 4 rows
             }
           }
-          if (row < rows) dst[(kStateGroups - 1) * rows + row] = make_float4(m_used, d_sum, 0.f, 0.f);
+          if (row < rows) dst[(kStateGroups - 1) * kGqa] = make_float4(m_used, d_sum, 0.f, 0.f);
         } else {
           // both streams hold states of the same rows: each group joins half of the columns
+          float4* const dst = state_row(r);
           exchange[s * kRows + r] = make_float2(m_used, d_sum);
           mbar_arrive(x_full);
           if (!wait_warp(x_full, uint32_t(nx) & 1u)) {
@@ -648,11 +653,11 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
             if (r < rows) {
 #pragma unroll
               for (int e = 0; e < 16; e += 4)
-                dst[((c0 + e) >> 2) * rows + r] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                dst[c0 + e] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
           }
           if (s == 0 && r < rows)
-            dst[(kStateGroups - 1) * rows + r] = make_float4(m, wa * a.y + (n1 > 0 ? wb * b.y : 0.f), 0.f, 0.f);
+            dst[(kStateGroups - 1) * kGqa] = make_float4(m, wa * a.y + (n1 > 0 ? wb * b.y : 0.f), 0.f, 0.f);
           tc::fence_before_sync();
           mbar_arrive(x_done);
           if (!wait_warp(x_done, uint32_t(nx) & 1u)) {
@@ -814,7 +819,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
           float d_row = d_run;
           d_row += __shfl_xor_sync(0xffffffffu, d_row, 1);
           d_row += __shfl_xor_sync(0xffffffffu, d_row, 2);
-          float* dst = p.own + ((int64_t(blockIdx.x + cur_b) * kNumKvHeads + h) * kOwnState + (gi & 3)) * 4;
+          float* dst = p.own + ((int64_t(blockIdx.x + cur_b) * kNumKvHeads + h) * kState + (gi & 3)) * 4;
 #pragma unroll
           for (int nt = 0; nt < 16; ++nt) {
             o[nt][0] += __shfl_xor_sync(0xffffffffu, o[nt][0], 16);
@@ -853,28 +858,22 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
 }
 
 constexpr int kJoinThreads = 128;  // one block per (request, kv head)
-constexpr int kJoinStates = 8;     // states at a time
-
-__device__ __forceinline__ float4 ld_state(const float4* p) {  // past L1, behind the wait (volatile)
-  float4 v;
-  asm volatile("ld.global.cg.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
-  return v;
-}
+constexpr int kMaxJoinStates = 24;
 
 // Joins the states of a request and kv head: of its own entries (one per CTA that holds a part of them) and of its
-// group's prefix (one per segment).  Thread = (row lane % 4, column group), so that four lanes read 64 consecutive
-// bytes; eight states at a time, each lane with (m, d) of one of them and a column group of all, the weights
-// passed by shuffle.  Bound by latency: what is known before the states is read before the wait, and the code is
-// short (unrolled over all states with two rows per warp it took 1 us per state, most of it instruction fetch).
-__global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_constant__ SharedPrefixParams p) {
-  const int lane = threadIdx.x & 31;
+// group's prefix (one per segment).  Bound by latency: what is known before the states is read before the wait,
+// every state is one bulk copy into shared memory, up to `room` of them in flight at once, and the code is short.
+// (Read by the threads themselves, 64 bytes per four lanes, 18 states took 9 us.)  Thread = (row, column group).
+__global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_constant__ SharedPrefixParams p, int room) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  float4* const in = reinterpret_cast<float4*>(smem);  // [room][kState]
+  uint64_t* const full = reinterpret_cast<uint64_t*>(smem + room * (kState * 16));
   const int b = blockIdx.x / kNumKvHeads, h = blockIdx.x % kNumKvHeads;
-  const int r = lane & 3, cg = threadIdx.x >> 2;  // row, column group
+  const int r = threadIdx.x & 3, cg = threadIdx.x >> 2;  // row, column group
   const float4* pre = reinterpret_cast<const float4*>(p.states);
-  const float4* own = reinterpret_cast<const float4*>(p.own) + h * kOwnState + r;
-  constexpr int64_t kOwnSeg = int64_t(kNumKvHeads) * kOwnState;
+  const float4* own = reinterpret_cast<const float4*>(p.own) + h * kState;
   int n_pre = 0, n_own = 0;
-  int64_t pitch = 0;
+  int64_t pre_step = 0;
   const int own_first = __ldg(p.indptr + b), own_last = __ldg(p.indptr + b + 1);
   const OwnSplit split(p);
   PlanView plan;
@@ -886,65 +885,69 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_
       const int4 job = ok ? __ldg(reinterpret_cast<const int4*>(plan.words + plan.job_at()) + req.x * kNumKvHeads + h)
                           : make_int4(0, 0, 0, 0);
       const int64_t off = uint32_t(job.x);
-      pitch = int64_t(kGqa) * job.z;
+      pre_step = int64_t(kState) * job.z;
       ok = ok && job.y >= 0 && job.z > 0 && job.z <= kBlockRequests && req.y >= 0 && req.y < job.z &&
-           off + int64_t(job.y) * kStateGroups * pitch <= p.state_size;
+           off + job.y * pre_step <= p.state_size;
       if (ok) {
-        pre += off + kGqa * req.y + r;
+        pre += off + req.y * kState;
         n_pre = job.y;
       }
     }
   }
   if (!ok && threadIdx.x == 0) atomicOr(p.status, kStatusBadLength);
   const int start = max(0, min(own_first, split.T)), end = max(start, min(own_last, split.T));
+  constexpr int64_t kOwnStep = int64_t(kNumKvHeads) * kState;
   if (end > start) {
     const int first = split.owner(start);
     n_own = split.owner(end - 1) - first + 1;
-    own += (first + int64_t(b)) * kOwnSeg;
+    own += (first + int64_t(b)) * kOwnStep;
   }
-  const int64_t pre_seg = kStateGroups * pitch;
+  if (threadIdx.x == 0) {
+    mbar_init(full, 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  // states 0 .. n_pre - 1 are the prefix's, the others the request's own; past the last one the last again
-  const int n = n_pre + n_own;
-  auto load = [&](int i, int group) {
-    i = min(i, n - 1);
-    return ld_state(i < n_pre ? pre + i * pre_seg + group * pitch : own + (i - n_pre) * kOwnSeg + group * kGqa);
-  };
+  const int n = n_pre + n_own;  // states 0 .. n_pre - 1 are the prefix's, the others the request's own
   float M = -INFINITY, D = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-  for (int i0 = 0; i0 < n; i0 += kJoinStates) {
-    const int mine = i0 + (lane >> 2);
-    float4 md = load(mine, kStateGroups - 1);
-    float4 v[kJoinStates];
-#pragma unroll
-    for (int e = 0; e < kJoinStates; ++e) v[e] = load(i0 + e, cg);
-    if (mine >= n) md.x = -INFINITY, md.y = 0.f;
-    float top = md.x;
-#pragma unroll
-    for (int d = 4; d <= 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    top = fmaxf(top, M);
-    const float w = md.x == -INFINITY ? 0.f : exp2f(md.x - top);
+  for (int i0 = 0, turn = 0; i0 < n; i0 += room, ++turn) {
+    const int have = min(room, n - i0);
+    if (threadIdx.x < 32) {
+      if (threadIdx.x == 0) mbar_arrive_expect_tx(full, uint32_t(have) * kState * 16);
+      __syncwarp();
+      for (int e = threadIdx.x; e < have; e += 32) {
+        const int i = i0 + e;
+        bulk_g2s(in + e * kState, i < n_pre ? pre + i * pre_step : own + (i - n_pre) * kOwnStep, kState * 16, full);
+      }
+    }
+    if (!mbar_wait_bounded(full, turn & 1)) {
+      atomicOr(p.status, kStatusWaitTimeout);
+      break;
+    }
+    const float4* const md = in + (kStateGroups - 1) * kGqa + r;
+    float top = M;
+#pragma unroll 4
+    for (int e = 0; e < have; ++e) top = fmaxf(top, md[e * kState].x);
     const float before = M == -INFINITY ? 0.f : exp2f(M - top);
     M = top;
-    float part = w * md.y;
-#pragma unroll
-    for (int d = 4; d <= 16; d <<= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
-    D = D * before + part;
+    D *= before;
     acc.x *= before;
     acc.y *= before;
     acc.z *= before;
     acc.w *= before;
-#pragma unroll
-    for (int e = 0; e < kJoinStates; ++e) {
-      const float we = __shfl_sync(0xffffffffu, w, 4 * e + r);
-      if (i0 + e >= n) continue;
-      acc.x += we * v[e].x;
-      acc.y += we * v[e].y;
-      acc.z += we * v[e].z;
-      acc.w += we * v[e].w;
+#pragma unroll 4
+    for (int e = 0; e < have; ++e) {
+      const float4 state = md[e * kState], v = in[e * kState + threadIdx.x];
+      const float w = state.x == -INFINITY ? 0.f : exp2f(state.x - M);
+      D += w * state.y;
+      acc.x += w * v.x;
+      acc.y += w * v.y;
+      acc.z += w * v.z;
+      acc.w += w * v.w;
     }
+    __syncthreads();  // before the next copies
   }
   const float inv = n > 0 ? 1.f / D : 0.f;  // no entries at all: output 0, LSE -inf
   const int row = h * kGqa + r;
@@ -1032,7 +1035,7 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
     w[4] = b.kv0 + segs[i].last;
     w[5] = int32_t(uint32_t(state));
     w[6] = flags | (b.len < kResidualMaxEntries ? kSegResidual : 0);
-    state += int64_t(kStateGroups) * kGqa * b.ntok;
+    state += int64_t(kState) * b.ntok;
   };
   int32_t* more = words + v.segment_at();
   for (int c = 0; c < ctas; ++c) {
@@ -1073,10 +1076,17 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
 }
 
 cudaError_t launch_shared_prefix_decode(const SharedPrefixParams& p, cudaStream_t stream) {
-  static std::atomic<uint64_t> configured{0};
+  static std::atomic<uint64_t> configured{0}, join_configured{0};
+  constexpr int kJoinState = kState * 16;
   if (cudaError_t e = set_max_dynamic_smem_once(shared_decode_kernel, kSmemBytes, configured)) return e;
+  if (cudaError_t e = set_max_dynamic_smem_once(shared_join_kernel, kMaxJoinStates * kJoinState + 16, join_configured))
+    return e;
   shared_decode_kernel<<<p.ctas, kThreads, kSmemBytes, stream>>>(p);
   if (cudaError_t e = cudaGetLastError()) return e;
+  // Room for the states that a request of an even batch has in one go (the loop takes any number): its prefix's,
+  // ctas / (8 blocks) and one, and its own, ctas / batch and two.  More room only keeps blocks from an SM.
+  const int blocks = (p.batch + kBlockRequests - 1) / kBlockRequests;
+  const int room = std::min(kMaxJoinStates, p.ctas / (kNumKvHeads * blocks) + 1 + p.ctas / p.batch + 2);
   // launched while the first kernel runs (programmatic stream serialization); it waits for its end itself
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1084,10 +1094,11 @@ cudaError_t launch_shared_prefix_decode(const SharedPrefixParams& p, cudaStream_
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(unsigned(p.batch) * kNumKvHeads);
   config.blockDim = dim3(kJoinThreads);
+  config.dynamicSmemBytes = size_t(room) * kJoinState + 16;
   config.stream = stream;
   config.attrs = &attr;
   config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, shared_join_kernel, p);
+  return cudaLaunchKernelEx(&config, shared_join_kernel, p, room);
 }
 
 }  // namespace dual

@@ -15,16 +15,17 @@ namespace dual {
 //   request  [requests][2]: block (-1: no prefix), place in the block
 //   job      [blocks x 8 kv heads][4]: offset of its first state (16-byte units), states, requests, 0
 // A block is up to 64 consecutive requests of one group; a job is a block and a kv head; its segments are
-// consecutive and split its prefix.  The state of a segment with n requests holds R = 4 n rows (request x
-// query head of the group): 33 groups of four floats, [group][row][4], 32 of unnormalised O and one of
-// (m, d, 0, 0), so that threads that own rows and threads that own columns both move whole sectors.
+// consecutive and split its prefix.  A state is that of one request and kv head, 33 groups of the 4 query heads'
+// four floats: 32 groups of unnormalised O and one of (m, d, 0, 0).  A segment's states follow one another by
+// request.  A thread that owns a row writes 16 bytes at a time, four threads whole sectors; the join reads a
+// state as one block.
 constexpr int kPlanMagic = 0x53505232;
 constexpr int kPlanHeader = 8;
 constexpr int kCtaWords = 12;
 constexpr int kSegmentWords = 8;
 constexpr int kBlockRequests = 64;    // requests of a block: two query tiles of 32 requests x 4 heads
 constexpr int kStateGroups = kHeadDim / 4 + 1;
-constexpr int kOwnState = kStateGroups * kGqa;  // state of one request's own entries in a CTA's range, 16-byte units
+constexpr int kState = kStateGroups * kGqa;  // 16-byte units
 constexpr int kSegResidual = 1;       // flags: P enters P V with its bf16 residual
 constexpr int kSegDeep = 2;           // no segment of this CTA has a second query tile: the ring has its room
 
@@ -83,7 +84,7 @@ struct SharedPrefixParams {
 
 // Workspace: [status: 256 B][own states: (CTAs + B) x 8 kv heads][prefix states].
 inline size_t shared_prefix_own_bytes(int batch, int ctas) {
-  return size_t(ctas + batch) * kNumKvHeads * kOwnState * 16;
+  return size_t(ctas + batch) * kNumKvHeads * kState * 16;
 }
 
 // Writes the plan (when `words` has room for it) and returns its size in words.

@@ -47,7 +47,7 @@ def test_segments_cover_every_prefix_once_and_states_do_not_overlap(seed):
     seen, places = {}, []
     for tok0, ntok, head, first, last, off, flags, _ in seg:
         assert first < last and 0 < ntok <= 64
-        places.append((off, off + 33 * 4 * ntok))
+        places.append((off, off + 132 * ntok))
         for t in range(tok0, tok0 + ntok):
             seen.setdefault((t, head), []).append((first, last, off, t - tok0, flags))
     places.sort()
@@ -65,7 +65,7 @@ def test_segments_cover_every_prefix_once_and_states_do_not_overlap(seed):
                 off, count, ntok, _ = job[block * 8 + h]
                 assert count == len(mine)
                 for i, m in enumerate(mine):
-                    assert m[2] == off + i * 33 * 4 * ntok and m[3] == local
+                    assert m[2] == off + i * 132 * ntok and m[3] == local
     assert ops.shared_prefix_workspace_size(plan) >= 16 * size + 8 * 132 * 16 * (gi[-1] + len(cta) - 1)
 
 
