@@ -102,13 +102,8 @@ struct Segment {
   int64_t state;  // 16-byte units
   bool single;    // one query tile, the streams take kv tiles in turn
   __device__ __forceinline__ int tiles() const { return (kv1 - kv0 + kBN - 1) / kBN; }
-  // kv tiles of stream s, and the i-th of them
-  __device__ __forceinline__ int tiles_of(int s) const { return single ? (tiles() + 1 - s) / 2 : tiles(); }
-  __device__ __forceinline__ int tile(int s, int i) const { return single ? 2 * i + s : i; }
-  // The ring holds tiles in the order in which the products take them.  Both streams on every tile:
-  // K0 V0 K1 V1 ...; tiles in turn: K0 K1 V0 K2 V1 K3 V2 ... (stream s needs K(t + 2) right after V(t)).
-  __device__ __forceinline__ int fill_of_k(int t) const { return !single ? 2 * t : t == 0 ? 0 : 2 * t - 1; }
-  __device__ __forceinline__ int fill_of_v(int t) const { return !single || t == tiles() - 1 ? 2 * t + 1 : 2 * t + 2; }
+  __device__ __forceinline__ int tiles_of(int s) const { return single ? (tiles() + 1 - s) / 2 : tiles(); }  // stream s
+  __device__ __forceinline__ int tile(int s, int i) const { return single ? 2 * i + s : i; }  // the i-th of them
 };
 
 // Segment `i` of CTA `cta` (of `count`; the second is at `second` among the segments); false (and a status bit)
@@ -116,7 +111,7 @@ struct Segment {
 __device__ __forceinline__ bool load_segment(const SharedPrefixParams& p, int second, int i, Segment& g) {
   const int32_t* at = i == 0 ? p.plan + kPlanHeader + int64_t(blockIdx.x) * kCtaWords + 4
                              : p.plan + kPlanHeader + int64_t(p.ctas) * kCtaWords + int64_t(second + i - 1) * kSegmentWords;
-  const int4 a = __ldg(reinterpret_cast<const int4*>(at)), b = __ldg(reinterpret_cast<const int4*>(at) + 1);
+  const int4 a = *reinterpret_cast<const int4*>(at), b = *(reinterpret_cast<const int4*>(at) + 1);
   g.tok0 = a.x;
   g.ntok = a.y;
   g.head = a.z;
@@ -215,8 +210,8 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // everything that the first loads depend on, in one round trip
-  const int4 cta_words = __ldg(reinterpret_cast<const int4*>(p.plan + kPlanHeader + int64_t(blockIdx.x) * kCtaWords));
-  const int first_flags = __ldg(p.plan + kPlanHeader + int64_t(blockIdx.x) * kCtaWords + 10);
+  const int4 cta_words = *reinterpret_cast<const int4*>(p.plan + kPlanHeader + int64_t(blockIdx.x) * kCtaWords);
+  const int first_flags = p.plan[kPlanHeader + int64_t(blockIdx.x) * kCtaWords + 10];
   const OwnSplit split(p);
   PlanView plan;
   bool planned = plan.open(p.plan, p.plan_words) && plan.ctas == p.ctas && plan.requests == p.batch;
@@ -334,7 +329,8 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
         int32_t next = page_of(0), after = ntiles > 1 ? page_of(1) : 0;
         const int fills = 2 * ntiles;
         for (int f = 0; f < fills; ++f) {
-          // which tile this is (the inverse of fill_of_k / fill_of_v)
+          // The ring holds tiles in the order in which the products take them.  Both streams on every tile:
+          // K0 V0 K1 V1 ...; tiles in turn: K0 K1 V0 K2 V1 K3 V2 ... (stream s needs K(t + 2) right after V(t)).
           const bool is_k = g.single ? f == 0 || ((f & 1) && f < fills - 1) : !(f & 1);
           const int t = !g.single ? f >> 1 : f == fills - 1 ? ntiles - 1 : is_k ? (f + 1) >> 1 : (f >> 1) - 1;
           const char* row;
@@ -386,91 +382,136 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
       asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == kMmaWarp) {
       // ============================================================== MMA issue
-      // The whole warp runs the loop in uniform control flow, one elected lane issues.
+      // The whole warp runs the loop in uniform control flow, one elected lane issues.  What the instructions'
+      // descriptors and addresses follow from stays in uniform registers: constants, loop counters, and what the
+      // plan says passed through a warp reduction (left as loaded, an instruction took 75 cycles to issue even to
+      // an idle tensor core, and the issue rate set the pace).
       const bool leader = tc::elect_one();
       constexpr uint32_t kIdescQK = tc::idesc_bf16_f32(128, kBN, 0, 0);
       constexpr uint32_t kIdescPV = tc::idesc_bf16_f32(128, 128, 0, 1);
       const uint32_t base = smem_addr(smem);
-      int u0 = 0, nq = 0;    // ring fills of the segments before, query tiles so far
-      int np0 = 0, np1 = 0;  // P tiles taken from each stream
-      auto slot_wait = [&](int f) { return wait_warp(slot_full + slot_of(u0 + f), uint32_t(turn_of(u0 + f)) & 1u); };
-      auto slot_free = [&](int f) {
-        if (leader) tc::commit(slot_empty + slot_of(u0 + f));
+      const int nslots = __reduce_max_sync(0xffffffffu, slots);
+      int pos = 0, turn = 0;     // the ring's next tile, in the order in which the products take them
+      int nq = 0;                // query tiles so far
+      uint32_t np0 = 0, np1 = 0;  // P tiles taken from each stream
+      auto advance = [&]() {
+        if (++pos == nslots) {
+          pos = 0;
+          ++turn;
+        }
+      };
+      auto slot_free = [&](int slot) {
+        if (leader) tc::commit(slot_empty + slot);
+      };
+      bool residual = false;
+      // O_s (+)= P_s V, in the two parts in which the softmax hands P over (entries 32..127, 0..31)
+      auto issue_pv = [&](int s, int slot, bool first) -> bool {
+        const uint32_t np = s == 0 ? np0 : np1;
+        const uint32_t v_base = base + slot_offset(slot);
+        const uint32_t tP = tmem + s * kBN, tO = tmem + kColO + s * 128;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          if (!wait_warp(p_part + 2 * s + part, np & 1u)) return false;
+          tc::fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < (part == 0 ? 6 : 2); ++k) {
+            const int kb = part == 0 ? 2 + k : k;
+            const uint64_t vdesc = tc::smem_desc_sw128(v_base + kb * 2048, kBN * 128, 1024);
+            const uint32_t ph = tP + 32 * (kb >> 1) + 8 * (kb & 1);
+            if (leader) {
+              tc::mma_bf16_ts(tO, ph, vdesc, kIdescPV, (!first || part > 0 || k > 0) ? 1u : 0u);
+              if (residual) tc::mma_bf16_ts(tO, ph + 16, vdesc, kIdescPV, 1u);
+            }
+          }
+        }
+        if (s == 0)
+          ++np0;
+        else
+          ++np1;
+        return true;
+      };
+      // S_s = Q K^T with query tile q
+      auto issue_qk = [&](int s, int slot, int q) {
+        const uint32_t qb = base + q * kQBytes, kb0 = base + slot_offset(slot);
+#pragma unroll
+        for (int kb = 0; kb < 8; ++kb) {
+          const uint32_t off_q = (kb >> 2) * (kRows * 128) + (kb & 3) * 32;
+          const uint32_t off_k = (kb >> 2) * (kBN * 128) + (kb & 3) * 32;
+          if (leader)
+            tc::mma_bf16(tmem + s * kBN, tc::smem_desc_sw128(qb + off_q, 16, 1024),
+                         tc::smem_desc_sw128(kb0 + off_k, 16, 1024), kIdescQK, kb > 0);
+        }
+        if (leader) tc::commit(s_full + s);  // S_s written, the PV before it done
+      };
+      // A tile has landed, and with it every earlier one of the ring: a loader thread arrives on a slot only once
+      // all of its earlier copies have landed.
+      auto landed = [&](int slot, int at) -> bool {
+        if (!wait_warp(slot_full + slot, uint32_t(at) & 1u)) return false;
+        fence_proxy_async_smem();  // cp.async writes -> tensor core reads
+        tc::fence_after_sync();
+        return true;
       };
       bool ok = true;
       for (int i = 0; i < nseg && ok; ++i) {
         Segment g;
         if (!load_segment(p, second, i, g)) continue;
-        const int ntiles = g.tiles(), steps = g.tiles_of(0);
-        const bool residual = (g.flags & kSegResidual) != 0;
-        // O_s (+)= P_s V(t), in the two parts in which the softmax hands P over (entries 32..127, 0..31)
-        auto issue_pv = [&](int s, int t, bool first) -> bool {
-          int& np = s == 0 ? np0 : np1;
-          const uint32_t v_base = base + slot_offset(slot_of(u0 + g.fill_of_v(t)));
-          const uint32_t tP = tmem + s * kBN, tO = tmem + kColO + s * 128;
-#pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            if (!wait_warp(p_part + 2 * s + part, uint32_t(np) & 1u)) return false;
-            tc::fence_after_sync();
-#pragma unroll
-            for (int k = 0; k < (part == 0 ? 6 : 2); ++k) {
-              const int kb = part == 0 ? 2 + k : k;
-              const uint64_t vdesc = tc::smem_desc_sw128(v_base + kb * 2048, kBN * 128, 1024);
-              const uint32_t ph = tP + 32 * (kb >> 1) + 8 * (kb & 1);
-              if (leader) {
-                tc::mma_bf16_ts(tO, ph, vdesc, kIdescPV, (!first || part > 0 || k > 0) ? 1u : 0u);
-                if (residual) tc::mma_bf16_ts(tO, ph + 16, vdesc, kIdescPV, 1u);
-              }
-            }
-          }
-          ++np;
-          return true;
-        };
+        const int ntiles = __reduce_max_sync(0xffffffffu, g.tiles());
+        const bool single = __reduce_max_sync(0xffffffffu, int(g.single)) != 0;
+        residual = __reduce_max_sync(0xffffffffu, g.flags & kSegResidual) != 0;
         ok = wait_warp(q_full, uint32_t(nq) & 1u);
-        for (int j = 0; j < steps && ok; ++j) {
-          for (int s = 0; s < kStreams && ok; ++s) {
-            const int t = g.tile(s, j);
-            if (t >= ntiles) break;  // the odd stream has one tile less
-            // K(t) landed, and with it every earlier tile of the ring: a loader thread arrives on a slot only
-            // once all of its earlier copies have landed
-            if (s == 0 || g.single) {
-              ok = slot_wait(g.fill_of_k(t));
-              if (!ok) break;
-              fence_proxy_async_smem();  // cp.async writes -> tensor core reads
-              tc::fence_after_sync();
-            }
-            if (j > 0) {
-              ok = issue_pv(s, g.tile(s, j - 1), j == 1);
-              if (!ok) break;
-              if (g.single || s == 1) slot_free(g.fill_of_v(g.tile(s, j - 1)));
-            }
-            const uint32_t qb = base + (g.single ? 0 : s) * kQBytes, kb0 = base + slot_offset(slot_of(u0 + g.fill_of_k(t)));
-#pragma unroll
-            for (int kb = 0; kb < 8; ++kb) {
-              const uint32_t off_q = (kb >> 2) * (kRows * 128) + (kb & 3) * 32;
-              const uint32_t off_k = (kb >> 2) * (kBN * 128) + (kb & 3) * 32;
-              if (leader)
-                tc::mma_bf16(tmem + s * kBN, tc::smem_desc_sw128(qb + off_q, 16, 1024),
-                             tc::smem_desc_sw128(kb0 + off_k, 16, 1024), kIdescQK, kb > 0);
-            }
-            if (leader) tc::commit(s_full + s);  // S_s written, the PV before it done
-            if (g.single || s == 1) slot_free(g.fill_of_k(t));
-          }
-        }
-        if (!ok) break;
-        if (leader) tc::commit(q_empty);
-        ok = slot_wait(2 * ntiles - 1);
-        if (ok) fence_proxy_async_smem();
-        for (int s = 0; s < kStreams && ok; ++s) {
-          const int n = g.tiles_of(s);
-          if (n == 0) continue;
-          ok = issue_pv(s, g.tile(s, n - 1), n == 1);
-          if (!ok) break;
-          if (leader) tc::commit(o_done + s);
-          if (g.single || s == 1) slot_free(g.fill_of_v(g.tile(s, n - 1)));
-        }
-        u0 += 2 * ntiles;
         ++nq;
+        if (single) {
+          for (int t = 0; t < ntiles && ok; ++t) {
+            const int s = t & 1, v = pos;
+            if (t >= 2) advance();
+            const int k = pos, at = turn;
+            advance();
+            ok = landed(k, at);
+            if (ok && t >= 2) {
+              ok = issue_pv(s, v, t < 4);
+              if (ok) slot_free(v);
+            }
+            if (!ok) break;
+            issue_qk(s, k, 0);
+            slot_free(k);
+          }
+          if (ok && leader) tc::commit(q_empty);
+          for (int t = max(0, ntiles - 2); t < ntiles && ok; ++t) {
+            const int s = t & 1, v = pos, at = turn;
+            advance();
+            ok = landed(v, at) && issue_pv(s, v, t < 2);
+            if (!ok) break;
+            if (leader) tc::commit(o_done + s);
+            slot_free(v);
+          }
+        } else {
+          for (int j = 0; j < ntiles && ok; ++j) {
+            const int v = pos;
+            if (j > 0) advance();
+            const int k = pos, at = turn;
+            advance();
+            ok = landed(k, at);
+#pragma unroll
+            for (int s = 0; s < kStreams; ++s) {
+              if (ok && j > 0) ok = issue_pv(s, v, j == 1);
+              if (!ok) break;
+              issue_qk(s, k, s);
+            }
+            if (!ok) break;
+            slot_free(k);
+            if (j > 0) slot_free(v);
+          }
+          if (ok && leader) tc::commit(q_empty);
+          const int v = pos, at = turn;
+          advance();
+          ok = ok && landed(v, at);
+#pragma unroll
+          for (int s = 0; s < kStreams; ++s) {
+            if (ok) ok = issue_pv(s, v, ntiles == 1);
+            if (ok && leader) tc::commit(o_done + s);
+          }
+          if (ok) slot_free(v);
+        }
       }
     } else {
       // ============================================================== softmax, a warpgroup per stream
