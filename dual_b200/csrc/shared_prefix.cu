@@ -1027,33 +1027,48 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
     }
   }
   const int32_t requests = groups > 0 ? group_indptr[groups] : 0;
-  // segments: CTA c owns units [c total / ctas, (c + 1) total / ctas) of the jobs laid end to end
+  // Segments: the jobs' units laid end to end, cut into one run per CTA.  A segment costs about a unit more than
+  // its units (its first tile's latency, its state), so a CTA whose run crosses into another job gets less: the
+  // smallest load M is sought with which runs of that load cover everything.
+  constexpr int64_t kSegmentUnits = 1;
   struct Seg {
     int32_t block, head, first, last;  // entries of the block's prefix
   };
   std::vector<Seg> segs;
   std::vector<int32_t> cta(size_t(ctas) + 1, 0);
   std::vector<int32_t> first_seg(blocks.size() * kNumKvHeads + 1, 0);
-  size_t job = 0;       // block x kv head
-  int64_t done = 0;     // units of that job that are given out
-  for (int c = 0; c < ctas; ++c) {
-    cta[c] = int32_t(segs.size());
-    int64_t want = (int64_t(c + 1) * total) / ctas - (int64_t(c) * total) / ctas;
-    while (want > 0) {
-      const Block& b = blocks[job / kNumKvHeads];
-      if (done == 0) first_seg[job] = int32_t(segs.size());
-      const int64_t take = std::min(want, b.units - done);
-      segs.push_back({int32_t(job / kNumKvHeads), int32_t(job % kNumKvHeads), int32_t(done * b.unit),
-                      int32_t(std::min<int64_t>((done + take) * b.unit, b.len))});
-      want -= take;
-      done += take;
-      if (done == b.units) {
-        done = 0;
-        ++job;
+  const size_t jobs = blocks.size() * kNumKvHeads;
+  auto deal = [&](int64_t load, bool keep) -> bool {
+    size_t job = 0;    // block x kv head
+    int64_t done = 0;  // units of that job that are given out
+    for (int c = 0; c < ctas; ++c) {
+      if (keep) cta[c] = int32_t(segs.size());
+      int64_t room = load;
+      while (job < jobs && room > kSegmentUnits) {
+        const Block& b = blocks[job / kNumKvHeads];
+        const int64_t take = std::min(room - kSegmentUnits, b.units - done);
+        if (keep) {
+          if (done == 0) first_seg[job] = int32_t(segs.size());
+          segs.push_back({int32_t(job / kNumKvHeads), int32_t(job % kNumKvHeads), int32_t(done * b.unit),
+                          int32_t(std::min<int64_t>((done + take) * b.unit, b.len))});
+        }
+        room -= take + kSegmentUnits;
+        done += take;
+        if (done == b.units) {
+          done = 0;
+          ++job;
+        }
       }
     }
+    return job == jobs;
+  };
+  int64_t low = kSegmentUnits, high = total + kSegmentUnits * int64_t(jobs) + 1;  // low is too little, high enough
+  while (high - low > 1) {
+    const int64_t mid = low + (high - low) / 2;
+    (deal(mid, false) ? high : low) = mid;
   }
-  cta[ctas] = first_seg[blocks.size() * kNumKvHeads] = int32_t(segs.size());
+  if (jobs > 0) deal(high, true);
+  cta[ctas] = first_seg[jobs] = int32_t(segs.size());
 
   PlanView v{};
   v.ctas = ctas;
@@ -1080,7 +1095,8 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
   };
   int32_t* more = words + v.segment_at();
   for (int c = 0; c < ctas; ++c) {
-    int32_t* w = words + kPlanHeader + int64_t(c) * kCtaWords;
+    // the last CTAs get the first runs: few own entries are in the first CTAs
+    int32_t* w = words + kPlanHeader + int64_t(ctas - 1 - c) * kCtaWords;
     w[0] = cta[c + 1] - cta[c];
     w[1] = int32_t((more - (words + v.segment_at())) / kSegmentWords);
     int32_t flags = kSegDeep;

@@ -14,7 +14,7 @@ def read(plan):
     at = 8 + 12 * ctas
     more = [w[at + 8 * i:at + 8 * i + 8] for i in range(segments)]
     cta, seg = [0], []
-    for c in range(ctas):  # a CTA's record holds its first segment, the others stand behind the records
+    for c in reversed(range(ctas)):  # a CTA's record holds its first segment, the others stand behind the records
         count, second, _, _, *first = w[8 + 12 * c:20 + 12 * c]
         mine = [first] + more[second:second + count - 1] if count else []
         assert len(mine) == count
@@ -70,12 +70,13 @@ def test_segments_cover_every_prefix_once_and_states_do_not_overlap(seed):
 
 
 def test_work_is_even():
-    """One long prefix over 148 CTAs: the ranges differ by one unit at most."""
+    """One long prefix over 148 CTAs: a CTA has its units and one more per segment, and no CTA more than the even share
+    rounded up, and one."""
     for batch, unit in ((16, 256), (64, 128), (200, 128)):
         plan = ops.shared_prefix_plan([0, batch], [0, 32768], 148)
         _, cta, seg, _, _ = read(plan)
-        loads = [sum(-(-(s[4] - s[3]) // (256 if s[1] <= 32 else 128)) for s in seg[a:b]) for a, b in zip(cta, cta[1:])]
-        assert max(loads) - min(loads) <= 1 and unit in (128, 256)
+        load = [sum(1 + -(-(s[4] - s[3]) // (256 if s[1] <= 32 else 128)) for s in seg[a:b]) for a, b in zip(cta, cta[1:])]
+        assert max(load) <= -(-sum(load) // 148) + 1, (batch, unit, max(load), sum(load) / 148)
 
 
 def test_plan_refusals():
