@@ -182,7 +182,8 @@ int dual_shared_prefix_plan(const int32_t* group_indptr_host, const int32_t* pre
   if (groups > 0 && (group_indptr_host[0] != 0 || prefix_indptr_host[0] != 0))
     return fail(DUAL_EINVAL, "group_indptr and prefix_indptr start at 0");
   try {
-    *num_words = dual::shared_prefix_plan(group_indptr_host, prefix_indptr_host, groups, num_ctas, plan_host, max_words);
+    *num_words =
+        dual::shared_prefix_plan(group_indptr_host, prefix_indptr_host, groups, num_ctas, plan_host, max_words);
   } catch (const std::exception& e) {
     return fail(DUAL_ENOSPACE, "shared-prefix plan: %s", e.what());
   }

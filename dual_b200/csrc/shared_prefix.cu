@@ -327,6 +327,19 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
         // row pointers of this lane's entry: K and V of the newest tile, V of the one before
         const char *kr = nullptr, *vr = nullptr, *vr_before = nullptr;
         int32_t next = page_of(0), after = ntiles > 1 ? page_of(1) : 0;
+        auto load_q = [&]() {  // the query tiles; rows past the block are zero
+          const int rows = g.single ? kRows : kStreams * kRows;
+#pragma unroll 1
+          for (int r = lt >> 4; r < rows; r += kLoadThreads / 16) {
+            const int tok = r / kGqa;
+            const bool there = tok < g.ntok;
+            const __nv_bfloat16* src = p.q + int64_t(g.tok0 + (there ? tok : 0)) * p.q_stride_tok +
+                                       int64_t(g.head * kGqa + r % kGqa) * p.q_stride_head + chunk * 8;
+            cp_async_16_zfill(smem + (r / kRows) * kQBytes + tc::sw128_offset<kRows>(r % kRows, chunk), src, there);
+          }
+          cp_async_mbar_arrive_noinc(q_full);
+        };
+        if (nq == 0) load_q();  // while the page ids are on their way
         const int fills = 2 * ntiles;
         for (int f = 0; f < fills; ++f) {
           // The ring holds tiles in the order in which the products take them.  Both streams on every tile:
@@ -358,24 +371,16 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
             cp_async_16_zfill(dst_tile + tc::sw128_offset<kBN>(kWarpEntries * lw + rr, chunk), src + off, rr < valid);
           }
           cp_async_mbar_arrive_noinc(slot_full + s);
-          if (f == 0) {
-            // the query tiles, behind the first K tile so that it is on its way while the last
-            // segment's products still read the old ones; rows past the block are zero
-            if (nq > 0 && !wait_warp(q_empty, uint32_t(nq - 1) & 1u)) {
+          if (f == 0 && nq > 0) {
+            // behind the first K tile, so that it is on its way while the last segment's products still read
+            // the old query tiles
+            if (!wait_warp(q_empty, uint32_t(nq - 1) & 1u)) {
               ok = false;
               break;
             }
-            ++nq;
-            const int rows = g.single ? kRows : kStreams * kRows;
-            for (int r = lt >> 4; r < rows; r += kLoadThreads / 16) {
-              const int tok = r / kGqa;
-              const bool there = tok < g.ntok;
-              const __nv_bfloat16* src = p.q + int64_t(g.tok0 + (there ? tok : 0)) * p.q_stride_tok +
-                                         int64_t(g.head * kGqa + r % kGqa) * p.q_stride_head + chunk * 8;
-              cp_async_16_zfill(smem + (r / kRows) * kQBytes + tc::sw128_offset<kRows>(r % kRows, chunk), src, there);
-            }
-            cp_async_mbar_arrive_noinc(q_full);
+            load_q();
           }
+          if (f == 0) ++nq;
         }
         u0 += fills;
       }

@@ -166,52 +166,69 @@ def shared_prefix_decode(q: torch.Tensor, k_local: torch.Tensor, v_local: torch.
     ``shared_prefix_plan`` on the device.  ``workspace``: ``shared_prefix_workspace_size`` bytes; its first word is the
     status word (``status_clear`` it before the first call), the rest may hold anything."""
     dev = q.get_device()
-    B = q.shape[0]
-    qt, ot = q.stride(), out.stride()
-    if q.dtype is not torch.bfloat16 or q.shape != (B, NUM_QO_HEADS, HEAD_DIM) or qt[2] != 1:
-        raise ValueError("q must be bf16 [B, 32, 128] with contiguous head_dim")
-    if out.dtype is not torch.bfloat16 or out.shape != q.shape or ot[2] != 1:
-        raise ValueError("out must be bf16 [B, 32, 128] with contiguous head_dim")
-    for t, name in ((kv_indptr, "kv_indptr"), (prefix_indices, "prefix_indices"), (unified_indices, "unified_indices"),
-                    (plan, "plan")):
+    for t, name in ((kv_indptr, "kv_indptr"), (plan, "plan")):
         if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.get_device() != dev:
             raise ValueError(f"{name} must be contiguous int32 [n] on q's device")
-    if kv_indptr.numel() < B + 1:
+    if kv_indptr.numel() < q.shape[0] + 1:
         raise ValueError("kv_indptr too short")
+    if not workspace.is_contiguous() or workspace.get_device() != dev:
+        raise ValueError("workspace must be contiguous and on q's device")
+    _shared_prefix_launch(q, k_local, v_local, local_capacity, peer_k, peer_v, prefix_indices, kv_indptr.data_ptr(),
+                          unified_indices, sm_scale, plan.data_ptr(), plan.numel(), out, lse, workspace.data_ptr(),
+                          workspace.numel() * workspace.element_size(), num_ctas or default_ctas(dev))
+
+
+def _shared_prefix_launch(q, k_local, v_local, local_capacity, peer_k, peer_v, prefix_indices, kv_indptr: int,
+                          unified_indices, sm_scale, plan: int, plan_words: int, out, lse, workspace: int,
+                          workspace_bytes: int, num_ctas: int) -> None:
+    """``shared_prefix_decode`` where the index pointer array, the plan and the workspace are the caller's own."""
+    dev = q.get_device()
+    shape, qt, ot = q.shape, q.stride(), out.stride()
+    B = shape[0]
+    if q.dtype is not torch.bfloat16 or shape != (B, NUM_QO_HEADS, HEAD_DIM) or qt[2] != 1:
+        raise ValueError("q must be bf16 [B, 32, 128] with contiguous head_dim")
+    if out.dtype is not torch.bfloat16 or out.shape != shape or ot[2] != 1:
+        raise ValueError("out must be bf16 [B, 32, 128] with contiguous head_dim")
+    if (prefix_indices.dtype is not torch.int32 or prefix_indices.dim() != 1 or not prefix_indices.is_contiguous()
+            or prefix_indices.get_device() != dev):
+        raise ValueError("prefix_indices must be contiguous int32 [n] on q's device")
+    if (unified_indices.dtype is not torch.int32 or unified_indices.dim() != 1 or not unified_indices.is_contiguous()
+            or unified_indices.get_device() != dev):
+        raise ValueError("unified_indices must be contiguous int32 [n] on q's device")
     if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (B, NUM_QO_HEADS) or not lse.is_contiguous()
                             or lse.get_device() != dev):
         raise ValueError("lse must be contiguous fp32 [B, 32] on q's device")
     ls = _pool_stride(k_local, "k_local")
-    if v_local.shape != k_local.shape or v_local.dtype is not k_local.dtype or v_local.stride() != k_local.stride():
+    if v_local.shape != k_local.shape or v_local.dtype is not torch.bfloat16 or v_local.stride() != k_local.stride():
         raise ValueError("k/v local pools must share a slot stride and a size")
     if not 0 <= local_capacity < k_local.shape[0]:
         raise ValueError("local_capacity must be a slot of the local pools")
-    if not out.get_device() == k_local.get_device() == v_local.get_device() == workspace.get_device() == dev:
-        raise ValueError("out, the pools and the workspace must be on q's device")
-    if not workspace.is_contiguous():
-        raise ValueError("workspace must be contiguous")
+    if not out.get_device() == k_local.get_device() == v_local.get_device() == dev:
+        raise ValueError("out and the pools must be on q's device")
     n = len(peer_k)
     if len(peer_v) != n:
         raise ValueError("peer_k / peer_v count mismatch")
-    pk, pv, ps, slots = (C.c_void_p * max(n, 1))(), (C.c_void_p * max(n, 1))(), 0, 0
     if n > 8:
         raise ValueError("at most 8 supplier banks")
+    pk = pv = None
+    ps = slots = 0
     if n:
-        ps, slots = _pool_stride(peer_k[0], "peer_k0"), peer_k[0].shape[0]
-        for i in range(n):
-            for t, name in ((peer_k[i], "peer_k"), (peer_v[i], "peer_v")):
-                if t.shape[0] != slots or _pool_stride(t, name) != ps or t.get_device() < 0:
+        bank = peer_k[0]
+        ps, slots, bshape, bstride = _pool_stride(bank, "peer_k0"), bank.shape[0], bank.shape, bank.stride()
+        for banks, name in ((peer_k, "peer_k"), (peer_v, "peer_v")):
+            for i, t in enumerate(banks):
+                if (t.dtype is not torch.bfloat16 or t.shape != bshape or t.stride() != bstride
+                        or (t.get_device() < 0) != (dev < 0)):
                     raise ValueError(f"{name}{i}: all supplier banks must share a size and a slot stride, on GPUs")
-            pk[i], pv[i] = peer_k[i].data_ptr(), peer_v[i].data_ptr()
+        pk, pv = (C.c_void_p * n)(*[t.data_ptr() for t in peer_k]), (C.c_void_p * n)(*[t.data_ptr() for t in peer_v])
     if dev < 0:
         raise ValueError(f"expected CUDA tensors, got {q.device}")
+    row = NUM_QO_HEADS * HEAD_DIM  # one request has no stride of its own
     _lib.check(_lib.load().dual_shared_prefix_decode(
-        q.data_ptr(), qt[0] if B > 1 else NUM_QO_HEADS * HEAD_DIM, qt[1], k_local.data_ptr(), v_local.data_ptr(), ls,
-        local_capacity, pk, pv, n, ps, slots, prefix_indices.data_ptr(), prefix_indices.numel(), kv_indptr.data_ptr(),
-        unified_indices.data_ptr(), unified_indices.numel(), B, sm_scale, plan.data_ptr(), plan.numel(), out.data_ptr(),
-        ot[0] if B > 1 else NUM_QO_HEADS * HEAD_DIM, ot[1], None if lse is None else lse.data_ptr(),
-        workspace.data_ptr(), workspace.numel() * workspace.element_size(), num_ctas or default_ctas(dev), dev,
-        _raw_stream(dev)))
+        q.data_ptr(), qt[0] if B > 1 else row, qt[1], k_local.data_ptr(), v_local.data_ptr(), ls, local_capacity, pk,
+        pv, n, ps, slots, prefix_indices.data_ptr(), prefix_indices.numel(), kv_indptr, unified_indices.data_ptr(),
+        unified_indices.numel(), B, sm_scale, plan, plan_words, out.data_ptr(), ot[0] if B > 1 else row, ot[1],
+        None if lse is None else lse.data_ptr(), workspace, workspace_bytes, num_ctas, dev, _raw_stream(dev)))
 
 
 def append_plan(qo_indptr, kv_indptr, causal: bool, remote_counts=None) -> torch.Tensor:
@@ -327,7 +344,7 @@ def set_kv_buffer(k_local: torch.Tensor, v_local: torch.Tensor, locations: torch
 
 
 def _rows(t: torch.Tensor, n: int, heads: int, name: str, device: int) -> Tuple[int, int]:
-    """(pointer, token stride) of ``t``, checked to be bf16 [n, heads, 128] with heads x dims contiguous on ``device``."""
+    """(pointer, token stride) of ``t``, checked to be bf16 [n, heads, 128], heads x dims contiguous, on ``device``."""
     st = t.stride()
     if not (t.dtype is torch.bfloat16 and t.shape == (n, heads, HEAD_DIM) and (n == 0 or st[1:] == (HEAD_DIM, 1))):
         raise ValueError(f"{name} must be bf16 [n, {heads}, 128] with heads x dims contiguous")
@@ -411,25 +428,6 @@ def rope_set_kv_buffer(k_local: torch.Tensor, v_local: torch.Tensor, locations: 
         op, os_, qw, kw, norm_eps, n, status.data_ptr(), dev, _raw_stream(dev)))
 
 
-def _state(t: torch.Tensor, T: int, name: str, device: int) -> Tuple[int, int, int, int]:
-    """(pointer, token stride, head stride, element size) of an attention state [T, 32, 128]."""
-    st = t.stride()
-    if not ((t.dtype is torch.bfloat16 or t.dtype is torch.float32)
-            and t.shape == (T, NUM_QO_HEADS, HEAD_DIM) and (T == 0 or st[2] == 1)):
-        raise ValueError(f"{name} must be bf16 or fp32 [T, 32, 128] with contiguous head_dim")
-    if t.get_device() != device:
-        raise ValueError(f"{name} must be on out's device")
-    return t.data_ptr(), st[0] if T > 1 else NUM_QO_HEADS * HEAD_DIM, st[1], t.element_size()
-
-
-def _state_lse(t: torch.Tensor, T: int, name: str, device: int) -> int:
-    if not (t.dtype is torch.float32 and t.shape == (T, NUM_QO_HEADS) and t.is_contiguous()):
-        raise ValueError(f"{name} must be contiguous fp32 [T, 32]")
-    if t.get_device() != device:
-        raise ValueError(f"{name} must be on out's device")
-    return t.data_ptr()
-
-
 def merge_attention_states(states: Sequence[torch.Tensor], lses: Sequence[torch.Tensor], out: torch.Tensor,
                            lse: Optional[torch.Tensor] = None) -> None:
     """Join 1 to 8 partial attention states of the same queries over disjoint keys (what
@@ -440,29 +438,47 @@ def merge_attention_states(states: Sequence[torch.Tensor], lses: Sequence[torch.
         raise ValueError("need 1 to 8 states, each with its lse")
     dev = out.get_device()
     T = out.shape[0]
-    op, ot, oh, oe = _state(out, T, "out", dev)
+    shape, lse_shape, row = (T, NUM_QO_HEADS, HEAD_DIM), (T, NUM_QO_HEADS), NUM_QO_HEADS * HEAD_DIM
+    st = out.stride()
+    if not ((out.dtype is torch.bfloat16 or out.dtype is torch.float32) and out.shape == shape
+            and (T == 0 or st[2] == 1)):
+        raise ValueError("out must be bf16 or fp32 [T, 32, 128] with contiguous head_dim")
+    op, ot, oh, oe = out.data_ptr(), st[0] if T > 1 else row, st[1], out.element_size()
     if oh < HEAD_DIM or ot < HEAD_DIM:
         raise ValueError("out must not repeat rows")
+    osize = oe * (oh * (NUM_QO_HEADS - 1) + HEAD_DIM)  # bytes from a token's first value to its last
+    oend = op + oe * (T - 1) * ot + osize
+    lp = None
+    if lse is not None:
+        if not (lse.dtype is torch.float32 and lse.shape == lse_shape and lse.is_contiguous()
+                and lse.get_device() == dev):
+            raise ValueError("lse must be contiguous fp32 [T, 32] on out's device")
+        lp = lse.data_ptr()
     dtype = states[0].dtype
+    e = 2 if dtype is torch.bfloat16 else 4
     ptrs, toks, heads, lptrs = (C.c_void_p * n)(), (C.c_int64 * n)(), (C.c_int64 * n)(), (C.c_void_p * n)()
-    lp = None if lse is None else _state_lse(lse, T, "lse", dev)
     for i in range(n):
-        s = states[i]
-        sp, tok, head, e = _state(s, T, f"states[{i}]", dev)
+        s, l = states[i], lses[i]
+        st = s.stride()
+        if not ((dtype is torch.bfloat16 or dtype is torch.float32) and s.shape == shape and (T == 0 or st[2] == 1)
+                and s.get_device() == dev):
+            raise ValueError(f"states[{i}] must be bf16 or fp32 [T, 32, 128] with contiguous head_dim on out's device")
         if s.dtype is not dtype:
             raise ValueError("states must share a type")
-        if (sp, tok, head, e) != (op, ot, oh, oe) and _overlap(
-                op, oe * ot, oe * (oh * (NUM_QO_HEADS - 1) + HEAD_DIM), sp, e * tok,
-                e * (head * (NUM_QO_HEADS - 1) + HEAD_DIM), T):
+        sp, tok, head = s.data_ptr(), st[0] if T > 1 else row, st[1]
+        if sp < oend and (sp, tok, head, e) != (op, ot, oh, oe) and _overlap(
+                op, oe * ot, osize, sp, e * tok, e * (head * (NUM_QO_HEADS - 1) + HEAD_DIM), T):
             raise ValueError("out must be one of the states or not overlap them")
-        l = _state_lse(lses[i], T, f"lses[{i}]", dev)
-        if lp is not None and l != lp and abs(l - lp) < T * NUM_QO_HEADS * 4:
+        if not (l.dtype is torch.float32 and l.shape == lse_shape and l.is_contiguous() and l.get_device() == dev):
+            raise ValueError(f"lses[{i}] must be contiguous fp32 [T, 32] on out's device")
+        a = l.data_ptr()
+        if lp is not None and a != lp and abs(a - lp) < T * NUM_QO_HEADS * 4:
             raise ValueError("lse must be one of the lses or not overlap them")
-        ptrs[i], toks[i], heads[i], lptrs[i] = sp, tok, head, l
+        ptrs[i], toks[i], heads[i], lptrs[i] = sp, tok, head, a
     if dev < 0:
         raise ValueError(f"expected CUDA tensors, got {out.device}")
-    _lib.check(_lib.load().dual_merge_attention_states(ptrs, toks, heads, lptrs, n, dtype is torch.float32, T, op, ot,
-                                                       oh, oe == 4, lp, dev, _raw_stream(dev)))
+    _lib.check(_lib.load().dual_merge_attention_states(ptrs, toks, heads, lptrs, n, e == 4, T, op, ot, oh, oe == 4, lp,
+                                                       dev, _raw_stream(dev)))
 
 
 def migrate_copy(local_planes: torch.Tensor, remote_planes: torch.Tensor, num_planes: int, num_banks: int,

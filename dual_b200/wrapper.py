@@ -157,7 +157,12 @@ class SharedPrefixDecodeWrapper:
         self._use_cuda_graph = use_cuda_graph
         self.device = float_workspace_buffer.device
         self._float_workspace = float_workspace_buffer
+        self._device_index = float_workspace_buffer.get_device()
         self._num_ctas = num_ctas or ops.default_ctas(self.device.index or 0)
+        if not float_workspace_buffer.is_contiguous():
+            raise ValueError("float_workspace_buffer must be contiguous")
+        self._ws_ptr = float_workspace_buffer.data_ptr()
+        self._ws_bytes = float_workspace_buffer.numel() * float_workspace_buffer.element_size()
         self._buffers = dict(indptr=paged_kv_indptr_buffer, indices=paged_kv_indices_buffer,
                              prefix=prefix_indices_buffer, plan=plan_buffer)
         for name, t in self._buffers.items():
@@ -195,13 +200,15 @@ class SharedPrefixDecodeWrapper:
         if self._use_cuda_graph and self._batch not in (None, batch):
             raise ValueError(f"CUDA graphs keep their batch: {self._batch}, got {batch}")
         need = ops.shared_prefix_workspace_size(words)
-        if self._float_workspace.numel() * self._float_workspace.element_size() < need:
+        if self._ws_bytes < need:
             raise ValueError(f"float_workspace_buffer too small: need {need} bytes")
         self._plan = self._fill("plan", words, non_blocking)
         self._prefix = self._fill("prefix", prefix_indices, non_blocking)
         self._indptr = self._fill("indptr", indptr, non_blocking)
         self._indices = self._fill("indices", indices, non_blocking)
         ops.status_clear(self._float_workspace)  # the caller's buffer may hold anything
+        self._plan_ptr, self._plan_words = self._plan.data_ptr(), self._plan.numel()
+        self._indptr_ptr = self._indptr.data_ptr()
         self._batch = batch
         self._sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(head_dim)
 
@@ -224,12 +231,15 @@ class SharedPrefixDecodeWrapper:
             prefix, indices, capacity, scale = self._prefix, self._indices, k.shape[0] - 1, self._sm_scale
         if q.shape[0] != B:
             raise ValueError(f"q has {q.shape[0]} rows but plan() was for batch {B}")
+        if q.get_device() != self._device_index:
+            raise ValueError(f"q must be on {self.device}")
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out = torch.empty_like(q)
         if return_lse and lse is None:
-            lse = torch.empty((B, ops.NUM_QO_HEADS), dtype=torch.float32, device=q.device)
-        ops.shared_prefix_decode(q, k, v, int(capacity), peer_k, peer_v, prefix, self._indptr, indices, float(scale),
-                                 self._plan, out, lse if return_lse else None, self._float_workspace, self._num_ctas)
+            lse = torch.empty((B, ops.NUM_QO_HEADS), dtype=torch.float32, device=self.device)
+        ops._shared_prefix_launch(q, k, v, int(capacity), peer_k, peer_v, prefix, self._indptr_ptr, indices,
+                                  float(scale), self._plan_ptr, self._plan_words, out, lse if return_lse else None,
+                                  self._ws_ptr, self._ws_bytes, self._num_ctas)
         return (out, lse) if return_lse else out
 
     run_return_lse = functools.partialmethod(run, return_lse=True)

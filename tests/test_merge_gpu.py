@@ -55,7 +55,7 @@ def make(T, n, dtype, seed, empty=True):
 
 
 @pytest.mark.parametrize("T,n", [(1, 1), (1, 2), (5, 2), (33, 3), (257, 8), (1000, 5)])
-@pytest.mark.parametrize("dtype,out_dtype", itertools.product([torch.bfloat16, torch.float32], repeat=2))
+@pytest.mark.parametrize("dtype,out_dtype", list(itertools.product([torch.bfloat16, torch.float32], repeat=2)))
 def test_merge_matches_64_bits(T, n, dtype, out_dtype):
     states, lses = make(T, n, dtype, seed=T + n)
     out = torch.empty((T, 32, 128), dtype=out_dtype, device=DEV)
