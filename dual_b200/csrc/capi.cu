@@ -231,8 +231,10 @@ int dual_shared_prefix_decode(const void* q, int64_t q_stride_token, int64_t q_s
         return fail(DUAL_EINVAL, "peer bank %d pointer null or not 16-byte aligned", i);
   }
   if (!(sm_scale > 0.0)) return fail(DUAL_EINVAL, "sm_scale must be positive");
-  if (plan_words < dual::kPlanHeader || !aligned16(plan)) return fail(DUAL_EINVAL, "plan must be a 16-byte aligned plan");
   if (num_ctas <= 0 || num_ctas > 65535) return fail(DUAL_EINVAL, "num_ctas must be the plan's");
+  // every CTA reads its record before the kernel knows whether the words are a plan for this call
+  if (plan_words < dual::kPlanHeader + int64_t(num_ctas) * dual::kCtaWords || !aligned16(plan))
+    return fail(DUAL_EINVAL, "plan must be 16-byte aligned and hold a plan for %d CTAs", num_ctas);
   const size_t head = 256 + dual::shared_prefix_own_bytes(batch, num_ctas);
   if (workspace_bytes < head)
     return fail(DUAL_ENOSPACE, "workspace too small: need at least %zu bytes, got %zu", head, workspace_bytes);

@@ -15,7 +15,7 @@ import math
 import pytest
 import torch
 
-from dual_b200 import SharedPrefixDecodeWrapper, ops
+from dual_b200 import SharedPrefixDecodeWrapper, _lib, ops
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
@@ -272,7 +272,7 @@ def test_a_plan_of_another_batch_is_recorded():
     assert int(big.view(torch.int32)[0]) == 0x10
     # words that are no plan: only the requests' own entries are seen
     ops.status_clear(ws)
-    ops.shared_prefix_decode(*args, torch.zeros(64, dtype=torch.int32, device=DEV), out, None, ws)
+    ops.shared_prefix_decode(*args, torch.zeros(1 << 12, dtype=torch.int32, device=DEV), out, None, ws)
     assert int(ws.view(torch.int32)[0]) == 0x10
     own = Case.__new__(Case)
     own.__dict__.update(c.__dict__)
@@ -281,6 +281,8 @@ def test_a_plan_of_another_batch_is_recorded():
     own.check(out, None)
     # a workspace without room for the prefix's states
     plan = c.plan()
+    with pytest.raises(_lib.DualError, match="plan for 148 CTAs"):  # fewer words than the CTAs' records
+        ops.shared_prefix_decode(*args, plan.to(DEV)[:1000], out, None, ws, 148)
     small = torch.zeros(ops.decode_workspace_size(4, ops.default_ctas(0)) + 1024, dtype=torch.uint8, device=DEV)
     ops.shared_prefix_decode(*args, plan.to(DEV), out, None, small)
     assert int(small.view(torch.int32)[0]) == 0x10

@@ -140,7 +140,7 @@ def test_c_abi_refusals_come_before_any_launch():
     two = (C.c_void_p * 8)(*[16] * 8)
 
     def call(q=256, qs=4096, qh=128, k=256, stride=2048, capacity=9, peers=0, pstride=2048, slots=4, prefix=16, n_prefix=4,
-             kv=16, idx=16, n_idx=4, batch=2, scale=0.1, plan=256, words=100, out=256, os=4096, oh=128, ws=256,
+             kv=16, idx=16, n_idx=4, batch=2, scale=0.1, plan=256, words=104, out=256, os=4096, oh=128, ws=256,
              bytes_=1 << 24, ctas=8):
         rc = lib.dual_shared_prefix_decode(q, qs, qh, k, 256, stride, capacity, two, two, peers, pstride, slots, prefix,
                                            n_prefix, kv, idx, n_idx, batch, scale, plan, words, out, os, oh, None, ws,
@@ -154,7 +154,7 @@ def test_c_abi_refusals_come_before_any_launch():
             (dict(stride=2040), 1, "slot stride"), (dict(capacity=-1), 1, "local_capacity"), (dict(qh=132), 1, "q/out"),
             (dict(out=264), 1, "q/out"), (dict(peers=2, pstride=1024), 1, "peer banks"), (dict(peers=1, slots=0), 1, "peer banks"),
             (dict(scale=0.0), 1, "sm_scale"), (dict(scale=float("nan")), 1, "sm_scale"), (dict(words=4), 1, "plan"),
-            (dict(plan=260), 1, "plan"), (dict(ctas=0), 1, "num_ctas"), (dict(bytes_=1000), 3, "workspace too small"),
+            (dict(plan=260), 1, "plan"), (dict(words=103), 1, "for 8 CTAs"), (dict(ctas=0), 1, "num_ctas"), (dict(bytes_=1000), 3, "workspace too small"),
             (dict(ws=320), 1, "256-byte")]:
         rc, msg = call(**change)
         assert rc == code and said in msg, (change, rc, msg)
