@@ -49,7 +49,8 @@ SIGNATURES = {
         VP, C.c_int,                           # status (nullable), num_ctas
         C.c_int, VP]),                         # device, stream
     "dual_decode_noalloc_status": (C.c_int, [U32P, C.c_int, VP]),
-    "dual_shared_prefix_plan": (C.c_int, [VP, VP, C.c_int, C.c_int, VP, C.c_int64, C.POINTER(C.c_int64)]),
+    "dual_shared_prefix_plan": (C.c_int, [
+        VP, VP, C.c_int, C.c_int, C.c_int64, VP, C.c_int64, C.POINTER(C.c_int64)]),
     "dual_shared_prefix_workspace_size": (C.c_int, [VP, C.c_int64, C.POINTER(C.c_size_t)]),
     "dual_shared_prefix_decode": (C.c_int, [
         VP, C.c_int64, C.c_int64,              # q, strides

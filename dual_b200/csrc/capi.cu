@@ -171,7 +171,7 @@ int dual_decode_workspace_reset(void* workspace, size_t workspace_bytes, int bat
 }
 
 int dual_shared_prefix_plan(const int32_t* group_indptr_host, const int32_t* prefix_indptr_host, int groups,
-                            int num_ctas, int32_t* plan_host, int64_t max_words, int64_t* num_words) {
+                            int num_ctas, int64_t own_entries, int32_t* plan_host, int64_t max_words, int64_t* num_words) {
   g_last_error.clear();
   if (groups < 0 || num_ctas <= 0 || num_ctas > 65535 || !num_words)
     return fail(DUAL_EINVAL, "bad shared-prefix plan arguments");
@@ -182,8 +182,8 @@ int dual_shared_prefix_plan(const int32_t* group_indptr_host, const int32_t* pre
   if (groups > 0 && (group_indptr_host[0] != 0 || prefix_indptr_host[0] != 0))
     return fail(DUAL_EINVAL, "group_indptr and prefix_indptr start at 0");
   try {
-    *num_words =
-        dual::shared_prefix_plan(group_indptr_host, prefix_indptr_host, groups, num_ctas, plan_host, max_words);
+    *num_words = dual::shared_prefix_plan(group_indptr_host, prefix_indptr_host, groups, num_ctas, own_entries,
+                                          plan_host, max_words);
   } catch (const std::exception& e) {
     return fail(DUAL_ENOSPACE, "shared-prefix plan: %s", e.what());
   }

@@ -14,9 +14,8 @@
 // Work.  Prefixes: a job is (block of up to 64 requests, kv head); the plan lays the jobs' kv tiles end to end
 // and cuts them into one equal range per CTA (one CTA per SM), so a CTA works on one or a few segments, each a
 // part of one job, and a long prefix of a small batch still fills the GPU.  Own entries: the flattened token
-// axis is cut into one range per CTA as in tiered_decode_kernel.  Every CTA does both, the prefix first.  (With
-// half of the CTAs in the other order, so that one part's products would overlap the other's loads, 256 requests
-// over 16,384 entries and up to 600 of their own took 201 us instead of 158.)  shared_join_kernel joins the states; it is launched beside the first and waits for its end.
+// axis is cut into one range per CTA as in tiered_decode_kernel.  Which CTAs do which part is the plan's: some the
+// prefixes and the others the own entries, or each both, the prefixes first.  shared_join_kernel joins the states; it is launched beside the first and waits for its end.
 //
 // Prefix phase, warp-specialised; two streams of 128 rows x 128 entries alternate on the tensor core, one in
 // softmax while the other is in its products:
@@ -128,17 +127,17 @@ __device__ __forceinline__ bool load_segment(const SharedPrefixParams& p, int se
   return ok;
 }
 
-// The requests' own entries: the flattened token axis [0, T) over G CTAs, CTA g owning [g T / G, (g + 1) T / G)
-// (positions are int32, as in indptr).  A CTA has a tile at least, so that a request is not cut into more states
-// than it has tiles.
+// The requests' own entries: the flattened token axis [0, T) over G of the plan's CTAs for them, CTA g owning
+// [g T / G, (g + 1) T / G) (positions are int32, as in indptr).  A CTA has a tile at least, so that a request is not
+// cut into more states than it has tiles.
 struct OwnSplit {
   int T, G;
   bool bad;
-  __device__ __forceinline__ OwnSplit(const SharedPrefixParams& p) {
-    T = __ldg(p.indptr + p.batch);
+  __device__ __forceinline__ OwnSplit(const SharedPrefixParams& p, int t, int ctas) {
+    T = t;  // indptr[batch]
     bad = T > p.num_indices || T < 0;
     if (bad) T = T < 0 ? 0 : int(p.num_indices);
-    G = max(1, min(p.ctas, T / Own::TILE));
+    G = max(1, min(ctas, T / Own::TILE));
   }
   __device__ __forceinline__ int begin(int g) const { return g >= G ? T : int((int64_t(g) * T) / G); }
   __device__ __forceinline__ int owner(int x) const { return int((int64_t(x + 1) * G - 1) / T); }
@@ -212,9 +211,10 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
   // everything that the first loads depend on, in one round trip
   const int4 cta_words = *reinterpret_cast<const int4*>(p.plan + kPlanHeader + int64_t(blockIdx.x) * kCtaWords);
   const int first_flags = p.plan[kPlanHeader + int64_t(blockIdx.x) * kCtaWords + 10];
-  const OwnSplit split(p);
+  const int total_own = __ldg(p.indptr + p.batch);
   PlanView plan;
   bool planned = plan.open(p.plan, p.plan_words) && plan.ctas == p.ctas && plan.requests == p.batch;
+  const OwnSplit split(p, total_own, planned ? plan.own_ctas : p.ctas);
   int nseg = cta_words.x;
   const int second = cta_words.y;
   planned = planned && nseg >= 0 && second >= 0 && (nseg <= 1 || second <= plan.segments - (nseg - 1));
@@ -921,9 +921,10 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_
   int n_pre = 0, n_own = 0;
   int64_t pre_step = 0;
   const int own_first = __ldg(p.indptr + b), own_last = __ldg(p.indptr + b + 1);
-  const OwnSplit split(p);
+  const int total_own = __ldg(p.indptr + p.batch);
   PlanView plan;
   bool ok = plan.open(p.plan, p.plan_words) && plan.ctas == p.ctas && plan.requests == p.batch;
+  const OwnSplit split(p, total_own, ok ? plan.own_ctas : p.ctas);
   if (ok) {
     const int2 req = __ldg(reinterpret_cast<const int2*>(plan.words + plan.request_at()) + b);
     if (req.x >= 0) {
@@ -1013,7 +1014,12 @@ constexpr int64_t kResidualMaxEntries = 1024;
 }
 
 int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_indptr, int groups, int ctas,
-                           int32_t* words, int64_t max_words) {
+                           int64_t own_entries, int32_t* words, int64_t max_words) {
+  // What a CTA takes, in ns, measured on a B200 with all CTAs at work: a prefix's first tile and last state; a
+  // segment's; a unit of two query tiles x 128 entries, of one x 256; own entries' first tile and last state; a
+  // tile of 16 of them.
+  constexpr int64_t kPrefixStart = 5000, kSegmentNs = 3000, kPairNs = 2400, kSingleNs = 2700, kOwnStart = 4000,
+                    kOwnTile = 1600;
   struct Block {
     int32_t tok0, ntok, kv0, len, unit;
     int64_t units;
@@ -1032,10 +1038,9 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
     }
   }
   const int32_t requests = groups > 0 ? group_indptr[groups] : 0;
-  // Segments: the jobs' units laid end to end, cut into one run per CTA.  A segment costs about a unit more than
-  // its units (its first tile's latency, its state), so a CTA whose run crosses into another job gets less: the
-  // smallest load M is sought with which runs of that load cover everything.
-  constexpr int64_t kSegmentUnits = 1;
+  // Segments: the jobs' units laid end to end, cut into one run per CTA; a segment costs something beside its
+  // units, so a CTA whose run crosses into another job gets less.  deal() fills CTAs up to a load and returns how
+  // many it needs.
   struct Seg {
     int32_t block, head, first, last;  // entries of the block's prefix
   };
@@ -1043,21 +1048,24 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
   std::vector<int32_t> cta(size_t(ctas) + 1, 0);
   std::vector<int32_t> first_seg(blocks.size() * kNumKvHeads + 1, 0);
   const size_t jobs = blocks.size() * kNumKvHeads;
-  auto deal = [&](int64_t load, bool keep) -> bool {
+  auto deal = [&](int64_t load, bool keep) -> int {
     size_t job = 0;    // block x kv head
     int64_t done = 0;  // units of that job that are given out
-    for (int c = 0; c < ctas; ++c) {
+    int c = 0;
+    for (; c < ctas && job < jobs; ++c) {
       if (keep) cta[c] = int32_t(segs.size());
-      int64_t room = load;
-      while (job < jobs && room > kSegmentUnits) {
+      int64_t room = load - kPrefixStart;
+      while (job < jobs) {
         const Block& b = blocks[job / kNumKvHeads];
-        const int64_t take = std::min(room - kSegmentUnits, b.units - done);
+        const int64_t unit = b.ntok <= kTileTok ? kSingleNs : kPairNs;
+        const int64_t take = std::min((room - kSegmentNs) / unit, b.units - done);
+        if (take <= 0) break;
         if (keep) {
           if (done == 0) first_seg[job] = int32_t(segs.size());
           segs.push_back({int32_t(job / kNumKvHeads), int32_t(job % kNumKvHeads), int32_t(done * b.unit),
                           int32_t(std::min<int64_t>((done + take) * b.unit, b.len))});
         }
-        room -= take + kSegmentUnits;
+        room -= take * unit + kSegmentNs;
         done += take;
         if (done == b.units) {
           done = 0;
@@ -1065,15 +1073,41 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
         }
       }
     }
-    return job == jobs;
+    if (keep) std::fill(cta.begin() + c, cta.end(), int32_t(segs.size()));
+    return job == jobs ? c : ctas + 1;
   };
-  int64_t low = kSegmentUnits, high = total + kSegmentUnits * int64_t(jobs) + 1;  // low is too little, high enough
-  while (high - low > 1) {
-    const int64_t mid = low + (high - low) / 2;
-    (deal(mid, false) ? high : low) = mid;
+  // CTAs that the own entries need to be done by `load`
+  const int64_t own_tiles = own_entries > 0 ? (own_entries + DecodeCfg::TILE - 1) / DecodeCfg::TILE : 0;
+  auto own_need = [&](int64_t load) -> int64_t {
+    if (own_tiles == 0) return 0;
+    const int64_t each = (load - kOwnStart) / kOwnTile;
+    return each <= 0 ? ctas + 1 : (own_tiles + each - 1) / each;
+  };
+  auto smallest = [&](auto&& fits) {  // load, by bisection
+    int64_t low = 0, high = kPrefixStart + int64_t(jobs) * kSegmentNs + total * kSingleNs + kOwnStart + own_tiles * kOwnTile;
+    while (high - low > 50) {
+      const int64_t mid = low + (high - low) / 2;
+      (fits(mid) ? high : low) = mid;
+    }
+    return high;
+  };
+  // Either every CTA does its part of the prefixes and then of the own entries, or some do the one and the others
+  // the other, each part's latencies then being paid by its own CTAs only: 16 requests over 32,768 entries and up
+  // to 256 own took 45.3 us the first way and 38.7 the second, 64 over 32,768 and up to 512 took 65.4 and 59.8.
+  int own_ctas = ctas;
+  if (jobs > 0) {
+    int64_t load = smallest([&](int64_t m) { return deal(m, false) <= ctas; });
+    if (own_tiles > 0) {
+      const int64_t both = load + kOwnStart + (own_tiles + ctas - 1) / ctas * kOwnTile;
+      const int64_t apart = smallest([&](int64_t m) { return deal(m, false) + own_need(m) <= ctas; });
+      if (deal(apart, false) + own_need(apart) <= ctas && apart < both) {
+        load = apart;
+        own_ctas = ctas - deal(apart, false);
+      }
+    }
+    deal(load, true);
   }
-  if (jobs > 0) deal(high, true);
-  cta[ctas] = first_seg[jobs] = int32_t(segs.size());
+  first_seg[jobs] = int32_t(segs.size());
 
   PlanView v{};
   v.ctas = ctas;
@@ -1134,6 +1168,7 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
   words[4] = v.blocks;
   words[5] = int32_t(uint32_t(state));
   words[6] = int32_t(state >> 32);
+  words[7] = own_ctas;
   return size;
 }
 

@@ -7,7 +7,7 @@ namespace dual {
 
 // The plan, one array of int32 words made on the host by shared_prefix_plan():
 //   header   [kPlanHeader]: kPlanMagic, CTAs, segments, requests, blocks, state size (two words, in 16-byte
-//            units, low word first), 0
+//            units, low word first), CTAs [0, this) take the requests' own entries
 //   CTA      [CTAs][kCtaWords]: segments of this CTA, place of its second one among the segments, 0, 0, and its
 //            first segment (so that a CTA's first loads depend on one load of the plan only)
 //   segment  [segments][kSegmentWords]: first request, requests, kv head, first and last + 1 entry of the prefix
@@ -19,7 +19,7 @@ namespace dual {
 // four floats: 32 groups of unnormalised O and one of (m, d, 0, 0).  A segment's states follow one another by
 // request.  A thread that owns a row writes 16 bytes at a time, four threads whole sectors; the join reads a
 // state as one block.
-constexpr int kPlanMagic = 0x53505232;
+constexpr int kPlanMagic = 0x53505233;
 constexpr int kPlanHeader = 8;
 constexpr int kCtaWords = 12;
 constexpr int kSegmentWords = 8;
@@ -31,7 +31,7 @@ constexpr int kSegDeep = 2;           // no segment of this CTA has a second que
 
 struct PlanView {
   const int32_t* words;
-  int ctas, segments, requests, blocks;
+  int ctas, segments, requests, blocks, own_ctas;
   int64_t state_size;  // 16-byte units
   __host__ __device__ int64_t segment_at() const { return kPlanHeader + int64_t(ctas) * kCtaWords; }
   __host__ __device__ int64_t request_at() const { return segment_at() + int64_t(segments) * kSegmentWords; }
@@ -47,7 +47,8 @@ struct PlanView {
     requests = a.w;
     blocks = b.x;
     state_size = int64_t(uint32_t(b.y)) | (int64_t(b.z) << 32);
-    return a.x == kPlanMagic && ctas > 0 && segments >= 0 && requests >= 0 && blocks >= 0 && state_size >= 0 && total() <= have;
+    own_ctas = b.w;
+    return a.x == kPlanMagic && ctas > 0 && own_ctas > 0 && own_ctas <= ctas && segments >= 0 && requests >= 0 && blocks >= 0 && state_size >= 0 && total() <= have;
   }
 };
 
@@ -87,9 +88,10 @@ inline size_t shared_prefix_own_bytes(int batch, int ctas) {
   return size_t(ctas + batch) * kNumKvHeads * kState * 16;
 }
 
-// Writes the plan (when `words` has room for it) and returns its size in words.
+// Writes the plan (when `words` has room for it) and returns its size in words.  `own_entries`: how many entries of
+// their own the requests have in all, for the balance (negative: not known).
 int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_indptr, int groups, int ctas,
-                           int32_t* words, int64_t max_words);
+                           int64_t own_entries, int32_t* words, int64_t max_words);
 cudaError_t launch_shared_prefix_decode(const SharedPrefixParams& p, cudaStream_t stream);
 
 }  // namespace dual

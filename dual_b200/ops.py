@@ -130,20 +130,22 @@ def _host_indptr(t, name: str) -> torch.Tensor:
     return t.to("cpu", torch.int32).contiguous()
 
 
-def shared_prefix_plan(group_indptr, prefix_indptr, num_ctas: int = 0) -> torch.Tensor:
+def shared_prefix_plan(group_indptr, prefix_indptr, num_ctas: int = 0, own_entries: int = -1) -> torch.Tensor:
     """Host-side work plan of a decode with shared prefixes, an int32 CPU tensor: requests
     ``group_indptr[g] .. group_indptr[g + 1]`` share the prefix of ``prefix_indptr[g + 1] - prefix_indptr[g]``
-    entries.  It stays valid while both do.  ``group_indptr`` / ``prefix_indptr``: host sequences or tensors."""
+    entries.  It stays valid while both do.  ``own_entries``: how many entries of their own the requests have in all,
+    if known; it only decides how many CTAs work on them.  ``group_indptr`` / ``prefix_indptr``: host sequences or
+    tensors."""
     gi, pi = _host_indptr(group_indptr, "group_indptr"), _host_indptr(prefix_indptr, "prefix_indptr")
     if gi.numel() != pi.numel():
         raise ValueError("group_indptr and prefix_indptr need one entry per group and one more")
     groups, ctas = gi.numel() - 1, int(num_ctas) or default_ctas(0)
     lib = _lib.load()
     n = C.c_int64(0)
-    _lib.check(lib.dual_shared_prefix_plan(gi.data_ptr(), pi.data_ptr(), groups, ctas, None, 0, C.byref(n)))
+    _lib.check(lib.dual_shared_prefix_plan(gi.data_ptr(), pi.data_ptr(), groups, ctas, own_entries, None, 0, C.byref(n)))
     plan = torch.empty(n.value, dtype=torch.int32)
-    _lib.check(lib.dual_shared_prefix_plan(gi.data_ptr(), pi.data_ptr(), groups, ctas, plan.data_ptr(), n.value,
-                                           C.byref(n)))
+    _lib.check(lib.dual_shared_prefix_plan(gi.data_ptr(), pi.data_ptr(), groups, ctas, own_entries, plan.data_ptr(),
+                                           n.value, C.byref(n)))
     return plan
 
 

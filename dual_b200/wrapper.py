@@ -185,16 +185,16 @@ class SharedPrefixDecodeWrapper:
     def plan(self, group_indptr, prefix_indptr, prefix_indices: torch.Tensor, indptr: torch.Tensor,
              indices: torch.Tensor, num_qo_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
              sm_scale: Optional[float] = None, non_blocking: bool = True) -> None:
-        """``group_indptr`` / ``prefix_indptr`` (host sequences or tensors) are read on the host; the index lists
-        and ``indptr`` are copied to the device."""
+        """``group_indptr`` / ``prefix_indptr`` (host sequences or tensors) and ``indptr``'s last entry are read on the
+        host; the index lists and ``indptr`` are copied to the device."""
         if (num_qo_heads, num_kv_heads, head_dim, page_size) != (ops.NUM_QO_HEADS, ops.NUM_KV_HEADS,
                                                                  ops.HEAD_DIM, 1):
             raise ValueError("dual_b200 decode is built for 32 q heads, 8 kv heads, head_dim 128, page_size 1")
         gi, pi = torch.as_tensor(group_indptr).to("cpu"), torch.as_tensor(prefix_indptr).to("cpu")
-        words = ops.shared_prefix_plan(gi, pi, self._num_ctas)
         batch = int(gi[-1])
         if indptr.numel() != batch + 1:
             raise ValueError(f"indptr is for {indptr.numel() - 1} requests, the groups hold {batch}")
+        words = ops.shared_prefix_plan(gi, pi, self._num_ctas, int(indptr[-1]))
         if prefix_indices.numel() < int(pi[-1]):
             raise ValueError("prefix_indices is shorter than the prefixes")
         if self._use_cuda_graph and self._batch not in (None, batch):

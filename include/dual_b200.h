@@ -135,8 +135,10 @@ int dual_decode_noalloc_status(uint32_t* value_out, int device, void* stream);
  * dual_shared_prefix_plan (host): from HOST copies of group_indptr and prefix_indptr ([groups + 1],
  * starting at 0; group_indptr[groups] is the batch), writes the work plan (int32 words) and returns its
  * size in *num_words (call with plan_host = NULL to size it).  The plan is copied to the device (16-byte
- * aligned) and stays valid while the groups and the prefixes' lengths do: a decode loop that appends to
- * the requests' own lists makes it once.  num_ctas: CTAs of both launches (dual_decode_default_ctas).
+ * aligned) and stays valid while the groups and the prefixes' lengths do.  own_entries: how many entries
+ * of their own the requests have in all (negative if not known); it decides how many CTAs work on them and
+ * nothing else, so a plan serves own lists of any length, best those of about that many entries.  num_ctas:
+ * CTAs of the first launch (dual_decode_default_ctas).
  * dual_shared_prefix_workspace_size (host): bytes that a call with this plan needs; a larger workspace
  * serves smaller plans.  Its first 256 bytes hold the status word (clear it with dual_status_clear before
  * the first call), the rest are partial states and may hold anything.
@@ -145,7 +147,7 @@ int dual_decode_noalloc_status(uint32_t* value_out, int device, void* stream);
  * DUAL_STATUS_BAD_LENGTH; the outputs are then not to be used.  Calls that share a workspace must not
  * overlap.  q, out: 16-byte aligned, element strides that are multiples of 8. */
 int dual_shared_prefix_plan(const int32_t* group_indptr_host, const int32_t* prefix_indptr_host, int groups,
-                            int num_ctas, int32_t* plan_host, int64_t max_words, int64_t* num_words);
+                            int num_ctas, int64_t own_entries, int32_t* plan_host, int64_t max_words, int64_t* num_words);
 int dual_shared_prefix_workspace_size(const int32_t* plan_host, int64_t plan_words, size_t* bytes);
 int dual_shared_prefix_decode(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_local,
                               const void* v_local, int64_t local_stride_bytes, int64_t local_capacity,

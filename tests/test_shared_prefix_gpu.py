@@ -65,11 +65,11 @@ class Case:
     def peers(self):
         return [t for pair in zip(self.bk, self.bv) for t in pair]
 
-    def plan(self, num_ctas=0):
-        return ops.shared_prefix_plan(self.gi, self.pi, num_ctas)
+    def plan(self, num_ctas=0, own=None):
+        return ops.shared_prefix_plan(self.gi, self.pi, num_ctas, sum(self.suffixes) if own is None else own)
 
-    def run(self, num_ctas=0, q=None, out=None, workspace=None):
-        plan = self.plan(num_ctas)
+    def run(self, num_ctas=0, q=None, out=None, workspace=None, own=None):
+        plan = self.plan(num_ctas, own)
         q = self.q if q is None else q
         B = q.shape[0]
         out = torch.full((B, 32, 128), 7.0, dtype=torch.bfloat16, device=DEV) if out is None else out
@@ -142,6 +142,15 @@ def test_any_number_of_ctas(num_ctas):
     """From one CTA that works on every job to more CTAs than units."""
     c = Case([5, 0, 40, 70], [700, 300, 1500, 129], mixed(115), banks=3, remote=0.2, seed=num_ctas)
     out, lse = c.run(num_ctas)
+    assert c.status == 0
+    c.check(out, lse)
+
+
+@pytest.mark.parametrize("own", [-1, 0, 5, 4000, 10 ** 7])
+def test_plans_for_other_own_lengths(own):
+    """The plan's idea of the own entries decides how many CTAs they get, not the result."""
+    c = Case([20, 60], [1100, 300], mixed(80), seed=17)
+    out, lse = c.run(own=own)
     assert c.status == 0
     c.check(out, lse)
 

@@ -11,6 +11,7 @@ from dual_b200 import SharedPrefixDecodeWrapper, _lib, ops
 def read(plan):
     w = plan.tolist()
     ctas, segments, requests, blocks = w[1:5]
+    assert 1 <= w[7] <= ctas
     at = 8 + 12 * ctas
     more = [w[at + 8 * i:at + 8 * i + 8] for i in range(segments)]
     cta, seg = [0], []
@@ -41,7 +42,7 @@ def test_segments_cover_every_prefix_once_and_states_do_not_overlap(seed):
     for s, p in zip(sizes, prefixes):
         gi.append(gi[-1] + s)
         pi.append(pi[-1] + p)
-    plan = ops.shared_prefix_plan(gi, pi, rng.choice([1, 3, 148]))
+    plan = ops.shared_prefix_plan(gi, pi, rng.choice([1, 2, 3, 20, 148]), rng.choice([-1, 0, 1, 300, 100000]))
     size, cta, seg, req, job = read(plan)
     assert cta[0] == 0 and cta[-1] == len(seg) and cta == sorted(cta) and len(req) == gi[-1]
     seen, places = {}, []
@@ -69,14 +70,33 @@ def test_segments_cover_every_prefix_once_and_states_do_not_overlap(seed):
     assert ops.shared_prefix_workspace_size(plan) >= 16 * size + 8 * 132 * 16 * (gi[-1] + len(cta) - 1)
 
 
-def test_work_is_even():
-    """One long prefix over 148 CTAs: a CTA has its units and one more per segment, and no CTA more than the even share
-    rounded up, and one."""
-    for batch, unit in ((16, 256), (64, 128), (200, 128)):
-        plan = ops.shared_prefix_plan([0, batch], [0, 32768], 148)
-        _, cta, seg, _, _ = read(plan)
-        load = [sum(1 + -(-(s[4] - s[3]) // (256 if s[1] <= 32 else 128)) for s in seg[a:b]) for a, b in zip(cta, cta[1:])]
-        assert max(load) <= -(-sum(load) // 148) + 1, (batch, unit, max(load), sum(load) / 148)
+def loads(plan):
+    """What each CTA has of the prefixes, in the planner's ns, and the CTAs that have own entries only."""
+    words = plan.tolist()
+    _, cta, seg, _, _ = read(plan)
+    ns = []
+    for a, b in zip(cta, cta[1:]):
+        units = lambda s: -(-(s[4] - s[3]) // (256 if s[1] <= 32 else 128)) * (2700 if s[1] <= 32 else 2400)  # noqa: E731
+        ns.append(5000 + sum(3000 + units(s) for s in seg[a:b]) if b > a else 0)
+    return ns, words[7]
+
+
+@pytest.mark.parametrize("batch,prefix", [(16, 32768), (64, 32768), (200, 32768), (300, 500)])
+def test_work_is_even(batch, prefix):
+    """No CTA has more than its start, the even share of what there is, a unit and a segment."""
+    ns, own = loads(ops.shared_prefix_plan([0, batch], [0, prefix], 148, 0))
+    assert own == 148 and max(ns) <= 5000 + sum(max(0, n - 5000) for n in ns) / 148 + 2700 + 3000
+
+
+@pytest.mark.parametrize("batch,prefix,entries", [(16, 32768, 2000), (64, 32768, 16000), (64, 4096, 2000), (3, 500, 60)])
+def test_own_entries_get_their_share_of_the_ctas(batch, prefix, entries):
+    """Apart from the prefixes' CTAs, and done at about the same time where there are many of them."""
+    ns, own = loads(ops.shared_prefix_plan([0, batch], [0, prefix], 148, entries))
+    assert own < 148 and all(n == 0 for n in sorted(ns)[:own])
+    tiles = -(-entries // 16)
+    assert 4000 + -(-tiles // own) * 1600 <= max(ns) + 1600
+    # not known: every CTA does both
+    assert loads(ops.shared_prefix_plan([0, batch], [0, prefix], 148))[1] == 148
 
 
 def test_plan_refusals():
@@ -98,7 +118,7 @@ def test_plan_refusals():
     # a list too short for the plan is left alone
     lib, n, few = _lib.load(), C.c_int64(0), torch.full((4,), -9, dtype=torch.int32)
     gi, pi = torch.tensor([0, 2], dtype=torch.int32), torch.tensor([0, 5], dtype=torch.int32)
-    assert lib.dual_shared_prefix_plan(gi.data_ptr(), pi.data_ptr(), 1, 8, few.data_ptr(), 4, C.byref(n)) == 0
+    assert lib.dual_shared_prefix_plan(gi.data_ptr(), pi.data_ptr(), 1, 8, -1, few.data_ptr(), 4, C.byref(n)) == 0
     assert n.value == good.numel() and few.tolist() == [-9] * 4
 
 
