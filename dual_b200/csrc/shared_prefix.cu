@@ -28,7 +28,7 @@
 // order in which the products take them, the MMA warp issues O_s += P_s V and S_s = Q K^T (P in tensor memory
 // over its own S), a softmax warpgroup per stream turns S into P with one thread per row; the running maximum
 // moves only when it grows by more than 2^8.
-// Own phase: one warp issues a bulk copy per row and plane (2 KiB, all kv heads), eight warps, one per kv head,
+// Own phase: K rows (2 KiB, all kv heads) come by bulk copies, V rows by 16-byte copies; eight warps, one per kv head,
 // multiply 16 entries at a time with the 4 query heads of the group as the rows of warp-level products.
 // All waits are bounded; one that runs out records DUAL_STATUS_WAIT_TIMEOUT and every role unwinds.
 #include <algorithm>
@@ -83,17 +83,19 @@ __device__ __forceinline__ void cp_async_16_zfill(void* dst, const void* src, bo
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(valid ? 16 : 0)
                : "memory");
 }
+__device__ __forceinline__ void cp_async_16_hint(void* dst, const void* src, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "l"(policy)
+               : "memory");
+}
 __device__ __forceinline__ void cp_async_mbar_arrive_noinc(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
-// D = A B + D where only rows 0..7 of the 16 x 16 A hold anything: the other rows' registers are zeros.
-__device__ __forceinline__ void mma_bf16_8x8x16(float* d, uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
-  float unused0, unused1;
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%9,%9};"
-      : "+f"(d[0]), "+f"(d[1]), "=f"(unused0), "=f"(unused1)
-      : "r"(a0), "r"(0u), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
+// An 8 x 8 matrix of 16-bit values (lane: row lane / 4, columns 2 (lane % 4) and + 1), transposed.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 
 struct Segment {
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
   uint64_t* q_empty = q_full + 1;                   // count 1 (tcgen05.commit, a segment's last QK)
   uint64_t* x_full = q_full + 2;                    // count kSoftmaxThreads: (m, d) of both streams written
   uint64_t* x_done = q_full + 3;                    // count kSoftmaxThreads: both streams' O read
-  uint64_t* own_full = q_full + 4;                  // [NS]     count 1 + bytes
+  uint64_t* own_full = q_full + 4;                  // [NS]     count 1 + 128 + bytes
   uint64_t* own_empty = own_full + Own::NS;         // [NS]     count 8
   uint64_t* ids_full = own_empty + Own::NS;         // [3]      count 32
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + kNumBars);
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
     mbar_init(x_full, kSoftmaxThreads);
     mbar_init(x_done, kSoftmaxThreads);
     for (int s = 0; s < Own::NS; ++s) {
-      mbar_init(own_full + s, 1);
+      mbar_init(own_full + s, 1 + 4 * 32);
       mbar_init(own_empty + s, Own::CONSUMERS);
     }
     for (int s = 0; s < Own::IDX_BUFS; ++s) mbar_init(ids_full + s, 32);
@@ -717,71 +719,87 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
   };
   // ---- own phase
   auto own_phase = [&]() {
-    if (warp == kSoftmaxWarps) {
+    int32_t* const sidx = reinterpret_cast<int32_t*>(smem + kOffIds);
+    constexpr int IC = Own::IDX_CHUNK, IB = Own::IDX_BUFS;
+    if (warp >= kSoftmaxWarps) {
       // ============================================================== row copies
+      // One warp stages the page ids and copies K rows, a bulk copy each; four copy V rows, 16 bytes per lane.  An
+      // SM takes about one bulk copy of 2 KiB per 60 cycles, so bulk copies alone held a tile to 1.5 us (77,000
+      // entries on half of the SMs: 108 us, this way 84).  The V rows, too, leave L2 first: without that hint all
+      // SMs together lost 6 % of the memory's rate.
+      const bool is_k = warp == kSoftmaxWarps;
+      const int chunk = tid - (kSoftmaxWarps + 1) * 32;  // of a V row, 0 .. 127
       OwnIter it;
       it.init(own_lo, own_hi, p.indptr, p.batch, lane);
-      int32_t* const sidx = reinterpret_cast<int32_t*>(smem + kOffIds);
-      constexpr int IC = Own::IDX_CHUNK, IB = Own::IDX_BUFS;
-      const int r = lane & 15;
-      const bool is_v = lane >= 16;
       const uint64_t policy = l2_policy_evict_first();
       const int nchunks = (own_hi - own_lo + IC - 1) / IC;
       int issued = 0, ready = -1;
-      auto issue_chunk = [&](int c) {
-        const int buf = c % IB;
-        const int first = own_lo + c * IC;
-        for (int i = lane; i < IC; i += 32)
-          if (first + i < own_hi) cp_async_4(sidx + buf * IC + i, p.indices + first + i);
-        cp_async_mbar_arrive_noinc(ids_full + buf);
+      auto issue_chunks = [&](int last) {  // of page ids
+        for (; issued < nchunks && issued <= last; ++issued) {
+          const int first = own_lo + issued * IC;
+          int32_t* const to = sidx + issued % IB * IC;
+          for (int i = lane; i < IC; i += 32)
+            if (first + i < own_hi) cp_async_4(to + i, p.indices + first + i);
+          cp_async_mbar_arrive_noinc(ids_full + issued % IB);
+        }
       };
-      while (issued < nchunks && issued < IB) issue_chunk(issued++);
-      int n_issued = 0;
-      for (; it.valid(); it.next(p.indptr, p.batch), ++n_issued) {
+      int n = 0;
+      for (; it.valid(); it.next(p.indptr, p.batch), ++n) {
         const int rows = it.rows();
         const int c_first = (it.t0 - own_lo) / IC, c_last = (it.t0 + rows - 1 - own_lo) / IC;
-        while (issued < nchunks && issued <= c_first + IB - 1) issue_chunk(issued++);
+        // the V warps are at most NS tiles behind: the chunk before this one may still be read, no earlier one
+        if (is_k) issue_chunks(c_first + IB - 2);
         bool ok = !*abort_flag;
         while (ok && ready < c_last) {
           ++ready;
           ok = wait(ids_full + (ready % IB), uint32_t(ready / IB) & 1u);
         }
-        const int stage = n_issued % Own::NS, fill = n_issued / Own::NS;
+        const int stage = n % Own::NS, fill = n / Own::NS;
         if (ok && fill > 0) ok = wait(own_empty + stage, uint32_t(fill - 1) & 1u);
         if (!__all_sync(0xffffffffu, ok)) break;
-        if (lane == 0) mbar_arrive_expect_tx(own_full + stage, uint32_t(rows) * 2u * Own::ROW_BYTES);
-        __syncwarp();
-        if (r < rows) {
-          const int off = it.t0 + r - own_lo;
-          const char *kr, *vr;
-          resolve(sidx[(off / IC) % IB * IC + off % IC], kr, vr);
-          bulk_g2s_hint(smem + stage * Own::STAGE_BYTES + (is_v ? Own::PLANE_BYTES : 0) + r * Own::PITCH, is_v ? vr : kr,
-                        Own::ROW_BYTES, own_full + stage, policy);
+        unsigned char* const to = smem + stage * Own::STAGE_BYTES;
+        const char *kr = nullptr, *vr = nullptr;  // of row `lane`
+        if (lane < rows) {
+          const int off = it.t0 + lane - own_lo;
+          resolve(sidx[off / IC % IB * IC + off % IC], kr, vr);
+        }
+        if (is_k) {
+          if (lane == 0) mbar_arrive_expect_tx(own_full + stage, uint32_t(rows) * Own::ROW_BYTES);
+          __syncwarp();
+          if (lane < rows) bulk_g2s_hint(to + lane * Own::PITCH, kr, Own::ROW_BYTES, own_full + stage, policy);
+        } else {
+#pragma unroll 4
+          for (int e = 0; e < rows; ++e)
+            cp_async_16_hint(to + Own::PLANE_BYTES + e * Own::PITCH + chunk * 16, shfl_ptr(vr, e) + chunk * 16, policy);
+          cp_async_mbar_arrive_noinc(own_full + stage);
         }
       }
       // never leave the phase with copies still landing in shared memory
       asm volatile("cp.async.wait_all;" ::: "memory");
-      for (int k = 0; k < min(n_issued, Own::NS); ++k) {
-        const int n = n_issued - 1 - k;
-        if (!mbar_wait_bounded(own_full + n % Own::NS, uint32_t(n / Own::NS) & 1u)) {
+      for (int k = 0; is_k && k < min(n, Own::NS); ++k) {
+        const int last = n - 1 - k;
+        if (!mbar_wait_bounded(own_full + last % Own::NS, uint32_t(last / Own::NS) & 1u)) {
           *abort_flag = 1;
           atomicOr(p.status, kStatusWaitTimeout);
           break;
         }
       }
-    } else if (warp < kSoftmaxWarps) {
+    } else {
       // ============================================================== products, a warp per kv head
+      // Scores and outputs are computed transposed, entries and dims being the rows of the 16 x 8 products and the
+      // query heads their columns: S^T = K Q^T, O^T += V^T P^T.  Columns 0..3 are the 4 heads of the group, 4..7
+      // the same heads again: P's high part goes into the first, its bf16 residual into the second, and their
+      // outputs are added when a state is written.  (With the heads as rows, 4 of 16, it took twice the products.)
       const int h = warp;
       const int gi = lane >> 2, ci = lane & 3;
+      const int mi = lane >> 3, rr = lane & 7;
       OwnIter it;
       it.init(own_lo, own_hi, p.indptr, p.batch, lane);
-      // Rows 0..3 of a product are the 4 query heads, rows 4..7 the same heads again: P's high part goes into
-      // the first, its bf16 residual into the second, and their outputs are added when a state is written.
-      uint32_t qa[8][2];
-      float o[16][2];
-      float m_run = -INFINITY, d_run = 0.f;
+      uint32_t qb[8][2];
+      float o[8][4];  // dims 16 d + gi and + 8, columns 2 ci and 2 ci + 1
+      float m0 = -INFINITY, m1 = -INFINITY, d0 = 0.f, d1 = 0.f;  // of those columns
 #pragma unroll
-      for (int nt = 0; nt < 16; ++nt) o[nt][0] = o[nt][1] = 0.f;
+      for (int d = 0; d < 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
       int cur_b = -1, n_seen = 0;
       for (; it.valid(); it.next(p.indptr, p.batch), ++n_seen) {
         if (it.b != cur_b) {
@@ -790,8 +808,8 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
               p.q + int64_t(cur_b) * p.q_stride_tok + int64_t(h * kGqa + (gi & 3)) * p.q_stride_head;
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
-            qa[ks][0] = *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 2 * ci);
-            qa[ks][1] = *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 8 + 2 * ci);
+            qb[ks][0] = *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 2 * ci);
+            qb[ks][1] = *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 8 + 2 * ci);
           }
         }
         const int stage = n_seen % Own::NS;
@@ -799,86 +817,97 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
         if (!wait_warp(own_full + stage, uint32_t(n_seen / Own::NS) & 1u)) break;
         const unsigned char* sK = smem + stage * Own::STAGE_BYTES + h * kHeadDim * 2;
         const unsigned char* sV = sK + Own::PLANE_BYTES;
-        const int mi = lane >> 3, rr = lane & 7;
-        // ---- S = Q K^T  (rows: 4 q heads, columns: 16 entries)
-        float s[2][2];
+        // ---- S^T, in two chains
+        float s[2][4] = {};
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          s[nt][0] = s[nt][1] = 0.f;
-#pragma unroll
-          for (int kp = 0; kp < 4; ++kp) {
-            uint32_t b0, b1, b2, b3;
-            ldmatrix_x4(b0, b1, b2, b3, sK + (nt * 8 + rr) * Own::PITCH + (kp * 32 + mi * 8) * 2);
-            mma_bf16_8x8x16(s[nt], qa[2 * kp][0], qa[2 * kp][1], b0, b1);
-            mma_bf16_8x8x16(s[nt], qa[2 * kp + 1][0], qa[2 * kp + 1][1], b2, b3);
-          }
+        for (int ks = 0; ks < 8; ++ks) {
+          uint32_t a0, a1, a2, a3;
+          ldmatrix_x4(a0, a1, a2, a3, sK + ((mi & 1) * 8 + rr) * Own::PITCH + (ks * 16 + (mi >> 1) * 8) * 2);
+          mma_bf16_16816(s[ks & 1], a0, a1, a2, a3, qb[ks][0], qb[ks][1]);
         }
         // ---- online softmax in the log2 domain; the running maximum moves only by more than 2^8
-        float x[4] = {s[0][0] * p.scale_log2, s[0][1] * p.scale_log2, s[1][0] * p.scale_log2, s[1][1] * p.scale_log2};
-        const int left = rows - 2 * ci;  // this lane's entries are 2 ci, 2 ci + 1 and the same + 8
-        if (left < 1) x[0] = -INFINITY;
-        if (left < 2) x[1] = -INFINITY;
-        if (left < 9) x[2] = -INFINITY;
-        if (left < 10) x[3] = -INFINITY;
-        float tmax = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-        tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 1));
-        tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 2));
-        float alpha = 1.f;
-        if (tmax > m_run + kRescaleThreshold) {
-          alpha = fast_exp2(m_run - tmax);  // 0 on a request's first tile
-          m_run = tmax;
+        float x[4];  // entries gi (two columns) and gi + 8
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = (s[0][e] + s[1][e]) * p.scale_log2;
+        if (gi >= rows) x[0] = x[1] = -INFINITY;
+        if (gi + 8 >= rows) x[2] = x[3] = -INFINITY;
+        float t0 = fmaxf(x[0], x[2]), t1 = fmaxf(x[1], x[3]);
+#pragma unroll
+        for (int d = 4; d <= 16; d <<= 1) {
+          t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, d));
+          t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, d));
+        }
+        float alpha0 = 1.f, alpha1 = 1.f;
+        if (t0 > m0 + kRescaleThreshold) {
+          alpha0 = fast_exp2(m0 - t0);  // 0 on a request's first tile
+          m0 = t0;
+        }
+        if (t1 > m1 + kRescaleThreshold) {
+          alpha1 = fast_exp2(m1 - t1);
+          m1 = t1;
         }
         float pr[4];
+        pr[0] = fast_exp2(x[0] - m0);
+        pr[1] = fast_exp2(x[1] - m1);
+        pr[2] = fast_exp2(x[2] - m0);
+        pr[3] = fast_exp2(x[3] - m1);
+        d0 = d0 * alpha0 + (pr[0] + pr[2]);
+        d1 = d1 * alpha1 + (pr[1] + pr[3]);
+        if (__any_sync(0xffffffffu, alpha0 != 1.f || alpha1 != 1.f)) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pr[e] = fast_exp2(x[e] - m_run);
-        d_run = d_run * alpha + (pr[0] + pr[1]) + (pr[2] + pr[3]);
-        if (__any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll
-          for (int nt = 0; nt < 16; ++nt) {
-            o[nt][0] *= alpha;
-            o[nt][1] *= alpha;
+          for (int d = 0; d < 8; ++d) {
+            o[d][0] *= alpha0;
+            o[d][1] *= alpha1;
+            o[d][2] *= alpha0;
+            o[d][3] *= alpha1;
           }
         }
         uint32_t hi0, hi2, lo0, lo2;
         split_bf16x2(pr[0], pr[1], hi0, lo0);
         split_bf16x2(pr[2], pr[3], hi2, lo2);
-        const uint32_t pa0 = gi < kGqa ? hi0 : lo0, pa2 = gi < kGqa ? hi2 : lo2;
-        // ---- O += P V; rows past the end hold whatever was there, and 0 x inf is not 0
+        const uint32_t b0 = transpose_8x8(ci < 2 ? hi0 : lo0), b1 = transpose_8x8(ci < 2 ? hi2 : lo2);
+        // ---- O^T += V^T P^T; rows past the end hold whatever was there, and 0 x inf is not 0
+        const int left = rows - 2 * ci;  // a lane's words are entries 2 ci, 2 ci + 1 and the same + 8
         const uint32_t keep0 = left > 1 ? ~0u : left == 1 ? 0xffffu : 0u;
         const uint32_t keep1 = left > 9 ? ~0u : left == 9 ? 0xffffu : 0u;
 #pragma unroll
-        for (int dp = 0; dp < 8; ++dp) {
-          uint32_t b0, b1, b2, b3;
-          ldmatrix_x4_trans(b0, b1, b2, b3, sV + ((mi & 1) * 8 + rr) * Own::PITCH + (dp * 16 + (mi >> 1) * 8) * 2);
+        for (int d = 0; d < 8; ++d) {
+          uint32_t a0, a1, a2, a3;
+          ldmatrix_x4_trans(a0, a1, a2, a3, sV + ((mi >> 1) * 8 + rr) * Own::PITCH + (d * 16 + (mi & 1) * 8) * 2);
           if (rows < Own::TILE) {
-            b0 &= keep0;
-            b1 &= keep1;
-            b2 &= keep0;
-            b3 &= keep1;
+            a0 &= keep0;
+            a1 &= keep0;
+            a2 &= keep1;
+            a3 &= keep1;
           }
-          mma_bf16_8x8x16(o[2 * dp], pa0, pa2, b0, b1);
-          mma_bf16_8x8x16(o[2 * dp + 1], pa0, pa2, b2, b3);
+          mma_bf16_16816(o[d], a0, a1, a2, a3, b0, b1);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(own_empty + stage);
         if (it.last_in_segment()) {
-          float d_row = d_run;
-          d_row += __shfl_xor_sync(0xffffffffu, d_row, 1);
-          d_row += __shfl_xor_sync(0xffffffffu, d_row, 2);
-          float* dst = p.own + ((int64_t(blockIdx.x + cur_b) * kNumKvHeads + h) * kState + (gi & 3)) * 4;
 #pragma unroll
-          for (int nt = 0; nt < 16; ++nt) {
-            o[nt][0] += __shfl_xor_sync(0xffffffffu, o[nt][0], 16);
-            o[nt][1] += __shfl_xor_sync(0xffffffffu, o[nt][1], 16);
-            if (gi < kGqa)
-              *reinterpret_cast<float2*>(dst + (nt * 2 + (ci >> 1)) * (kGqa * 4) + (ci & 1) * 2) =
-                  make_float2(o[nt][0], o[nt][1]);
-            o[nt][0] = o[nt][1] = 0.f;
+          for (int d = 4; d <= 16; d <<= 1) {
+            d0 += __shfl_xor_sync(0xffffffffu, d0, d);
+            d1 += __shfl_xor_sync(0xffffffffu, d1, d);
           }
-          if (gi < kGqa && ci == 0)
-            *reinterpret_cast<float2*>(dst + (kStateGroups - 1) * (kGqa * 4)) = make_float2(m_run, d_row);
-          m_run = -INFINITY;
-          d_run = 0.f;
+          // lanes ci and ci + 2 have a head pair's high and residual outputs: the first writes head 2 ci, the
+          // second head 2 ci + 1
+          const int head = 2 * (ci & 1) + (ci >> 1);
+          float* dst = p.own + (int64_t(blockIdx.x + cur_b) * kNumKvHeads + h) * (kState * 4) + head * 4 + (gi & 3) +
+                       (gi >> 2) * (kGqa * 4);
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[d][e] += __shfl_xor_sync(0xffffffffu, o[d][e], 2);
+            dst[(4 * d) * (kGqa * 4)] = ci < 2 ? o[d][0] : o[d][1];
+            dst[(4 * d + 2) * (kGqa * 4)] = ci < 2 ? o[d][2] : o[d][3];
+            o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+          }
+          if (gi == 0)
+            *reinterpret_cast<float2*>(dst + (kStateGroups - 1) * (kGqa * 4)) =
+                ci < 2 ? make_float2(m0, d0) : make_float2(m1, d1);
+          m0 = m1 = -INFINITY;
+          d0 = d1 = 0.f;
         }
       }
     }
@@ -1017,9 +1046,9 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
                            int64_t own_entries, int32_t* words, int64_t max_words) {
   // What a CTA takes, in ns, measured on a B200 with all CTAs at work: a prefix's first tile and last state; a
   // segment's; a unit of two query tiles x 128 entries, of one x 256; own entries' first tile and last state; a
-  // tile of 16 of them.
+  // tile of 16 of them; a request's state.
   constexpr int64_t kPrefixStart = 5000, kSegmentNs = 3000, kPairNs = 2400, kSingleNs = 2700, kOwnStart = 4000,
-                    kOwnTile = 1600;
+                    kOwnTile = 1100, kOwnRequest = 700;
   struct Block {
     int32_t tok0, ntok, kv0, len, unit;
     int64_t units;
@@ -1076,15 +1105,16 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
     if (keep) std::fill(cta.begin() + c, cta.end(), int32_t(segs.size()));
     return job == jobs ? c : ctas + 1;
   };
-  // CTAs that the own entries need to be done by `load`
-  const int64_t own_tiles = own_entries > 0 ? (own_entries + DecodeCfg::TILE - 1) / DecodeCfg::TILE : 0;
+  // CTAs that the own entries need to be done by `load`; a request's last tile is half full on average
+  const int64_t own_ns = own_entries <= 0 ? 0
+                                          : (own_entries / DecodeCfg::TILE + requests / 2 + 1) * kOwnTile +
+                                                requests * kOwnRequest;
   auto own_need = [&](int64_t load) -> int64_t {
-    if (own_tiles == 0) return 0;
-    const int64_t each = (load - kOwnStart) / kOwnTile;
-    return each <= 0 ? ctas + 1 : (own_tiles + each - 1) / each;
+    if (own_ns == 0) return 0;
+    return load <= kOwnStart ? ctas + 1 : (own_ns + load - kOwnStart - 1) / (load - kOwnStart);
   };
   auto smallest = [&](auto&& fits) {  // load, by bisection
-    int64_t low = 0, high = kPrefixStart + int64_t(jobs) * kSegmentNs + total * kSingleNs + kOwnStart + own_tiles * kOwnTile;
+    int64_t low = 0, high = kPrefixStart + int64_t(jobs) * kSegmentNs + total * kSingleNs + kOwnStart + own_ns;
     while (high - low > 50) {
       const int64_t mid = low + (high - low) / 2;
       (fits(mid) ? high : low) = mid;
@@ -1093,12 +1123,12 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
   };
   // Either every CTA does its part of the prefixes and then of the own entries, or some do the one and the others
   // the other, each part's latencies then being paid by its own CTAs only: 16 requests over 32,768 entries and up
-  // to 256 own took 45.3 us the first way and 38.7 the second, 64 over 32,768 and up to 512 took 65.4 and 59.8.
+  // to 256 own took 45.3 us the first way and 38.7 the second, 64 over 32,768 and up to 512 took 65.4 and 54.7.
   int own_ctas = ctas;
   if (jobs > 0) {
     int64_t load = smallest([&](int64_t m) { return deal(m, false) <= ctas; });
-    if (own_tiles > 0) {
-      const int64_t both = load + kOwnStart + (own_tiles + ctas - 1) / ctas * kOwnTile;
+    if (own_ns > 0) {
+      const int64_t both = load + kOwnStart + own_ns / ctas;
       const int64_t apart = smallest([&](int64_t m) { return deal(m, false) + own_need(m) <= ctas; });
       if (deal(apart, false) + own_need(apart) <= ctas && apart < both) {
         load = apart;

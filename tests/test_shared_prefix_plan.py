@@ -93,8 +93,8 @@ def test_own_entries_get_their_share_of_the_ctas(batch, prefix, entries):
     """Apart from the prefixes' CTAs, and done at about the same time where there are many of them."""
     ns, own = loads(ops.shared_prefix_plan([0, batch], [0, prefix], 148, entries))
     assert own < 148 and all(n == 0 for n in sorted(ns)[:own])
-    tiles = -(-entries // 16)
-    assert 4000 + -(-tiles // own) * 1600 <= max(ns) + 1600
+    own_ns = (entries // 16 + batch // 2 + 1) * 1100 + batch * 700
+    assert 4000 + own_ns / own <= max(ns) + 3000 + 2700
     # not known: every CTA does both
     assert loads(ops.shared_prefix_plan([0, batch], [0, prefix], 148))[1] == 148
 
