@@ -1045,13 +1045,13 @@ constexpr int64_t kResidualMaxEntries = 1024;
 int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_indptr, int groups, int ctas,
                            int64_t own_entries, int32_t* words, int64_t max_words) {
   // What a CTA takes, in ns, measured on a B200 with all CTAs at work: a prefix's first tile and last state; a
-  // segment's; a unit of two query tiles x 128 entries, of one x 256; own entries' first tile and last state; a
-  // tile of 16 of them; a request's state.
-  constexpr int64_t kPrefixStart = 5000, kSegmentNs = 3000, kPairNs = 2400, kSingleNs = 2700, kOwnStart = 4000,
+  // segment's; a kv tile with two query tiles, with one; own entries' first tile and last state; a tile of 16 of
+  // them; a request's state.
+  constexpr int64_t kPrefixStart = 5000, kSegmentNs = 3000, kPairNs = 2400, kSingleNs = 1350, kOwnStart = 4000,
                     kOwnTile = 1100, kOwnRequest = 700;
   struct Block {
-    int32_t tok0, ntok, kv0, len, unit;
-    int64_t units;
+    int32_t tok0, ntok, kv0, len;
+    int64_t tiles;
   };
   std::vector<Block> blocks;
   int64_t total = 0;
@@ -1060,15 +1060,13 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
     if (len == 0) continue;
     for (int32_t t = group_indptr[g]; t < group_indptr[g + 1]; t += kBlockRequests) {
       const int32_t ntok = std::min<int32_t>(kBlockRequests, group_indptr[g + 1] - t);
-      // a unit is what takes one softmax of both streams: 128 entries of two query tiles, 256 of one
-      const int32_t unit = ntok <= kTileTok ? 2 * kBN : kBN;
-      blocks.push_back({t, ntok, prefix_indptr[g], len, unit, (int64_t(len) + unit - 1) / unit});
-      total += blocks.back().units * kNumKvHeads;
+      blocks.push_back({t, ntok, prefix_indptr[g], len, (int64_t(len) + kBN - 1) / kBN});
+      total += blocks.back().tiles * kNumKvHeads;
     }
   }
   const int32_t requests = groups > 0 ? group_indptr[groups] : 0;
-  // Segments: the jobs' units laid end to end, cut into one run per CTA; a segment costs something beside its
-  // units, so a CTA whose run crosses into another job gets less.  deal() fills CTAs up to a load and returns how
+  // Segments: the jobs' kv tiles laid end to end, cut into one run per CTA; a segment costs something beside its
+  // tiles, so a CTA whose run crosses into another job gets less.  deal() fills CTAs up to a load and returns how
   // many it needs.
   struct Seg {
     int32_t block, head, first, last;  // entries of the block's prefix
@@ -1079,24 +1077,24 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
   const size_t jobs = blocks.size() * kNumKvHeads;
   auto deal = [&](int64_t load, bool keep) -> int {
     size_t job = 0;    // block x kv head
-    int64_t done = 0;  // units of that job that are given out
+    int64_t done = 0;  // tiles of that job that are given out
     int c = 0;
     for (; c < ctas && job < jobs; ++c) {
       if (keep) cta[c] = int32_t(segs.size());
       int64_t room = load - kPrefixStart;
       while (job < jobs) {
         const Block& b = blocks[job / kNumKvHeads];
-        const int64_t unit = b.ntok <= kTileTok ? kSingleNs : kPairNs;
-        const int64_t take = std::min((room - kSegmentNs) / unit, b.units - done);
+        const int64_t each = b.ntok <= kTileTok ? kSingleNs : kPairNs;
+        const int64_t take = std::min((room - kSegmentNs) / each, b.tiles - done);
         if (take <= 0) break;
         if (keep) {
           if (done == 0) first_seg[job] = int32_t(segs.size());
-          segs.push_back({int32_t(job / kNumKvHeads), int32_t(job % kNumKvHeads), int32_t(done * b.unit),
-                          int32_t(std::min<int64_t>((done + take) * b.unit, b.len))});
+          segs.push_back({int32_t(job / kNumKvHeads), int32_t(job % kNumKvHeads), int32_t(done * kBN),
+                          int32_t(std::min<int64_t>((done + take) * kBN, b.len))});
         }
-        room -= take * unit + kSegmentNs;
+        room -= take * each + kSegmentNs;
         done += take;
-        if (done == b.units) {
+        if (done == b.tiles) {
           done = 0;
           ++job;
         }
@@ -1114,7 +1112,7 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
     return load <= kOwnStart ? ctas + 1 : (own_ns + load - kOwnStart - 1) / (load - kOwnStart);
   };
   auto smallest = [&](auto&& fits) {  // load, by bisection
-    int64_t low = 0, high = kPrefixStart + int64_t(jobs) * kSegmentNs + total * kSingleNs + kOwnStart + own_ns;
+    int64_t low = 0, high = kPrefixStart + int64_t(jobs) * kSegmentNs + total * kPairNs + kOwnStart + own_ns;
     while (high - low > 50) {
       const int64_t mid = low + (high - low) / 2;
       (fits(mid) ? high : low) = mid;

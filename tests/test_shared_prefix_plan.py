@@ -76,16 +76,16 @@ def loads(plan):
     _, cta, seg, _, _ = read(plan)
     ns = []
     for a, b in zip(cta, cta[1:]):
-        units = lambda s: -(-(s[4] - s[3]) // (256 if s[1] <= 32 else 128)) * (2700 if s[1] <= 32 else 2400)  # noqa: E731
-        ns.append(5000 + sum(3000 + units(s) for s in seg[a:b]) if b > a else 0)
+        tiles = lambda s: -(-(s[4] - s[3]) // 128) * (1350 if s[1] <= 32 else 2400)  # noqa: E731
+        ns.append(5000 + sum(3000 + tiles(s) for s in seg[a:b]) if b > a else 0)
     return ns, words[7]
 
 
 @pytest.mark.parametrize("batch,prefix", [(16, 32768), (64, 32768), (200, 32768), (300, 500)])
 def test_work_is_even(batch, prefix):
-    """No CTA has more than its start, the even share of what there is, a unit and a segment."""
+    """No CTA has more than its start, the even share of what there is, a tile and a segment."""
     ns, own = loads(ops.shared_prefix_plan([0, batch], [0, prefix], 148, 0))
-    assert own == 148 and max(ns) <= 5000 + sum(max(0, n - 5000) for n in ns) / 148 + 2700 + 3000
+    assert own == 148 and max(ns) <= 5000 + sum(max(0, n - 5000) for n in ns) / 148 + 2400 + 3000
 
 
 @pytest.mark.parametrize("batch,prefix,entries", [(16, 32768, 2000), (64, 32768, 16000), (64, 4096, 2000), (3, 500, 60)])
@@ -94,7 +94,7 @@ def test_own_entries_get_their_share_of_the_ctas(batch, prefix, entries):
     ns, own = loads(ops.shared_prefix_plan([0, batch], [0, prefix], 148, entries))
     assert own < 148 and all(n == 0 for n in sorted(ns)[:own])
     own_ns = (entries // 16 + batch // 2 + 1) * 1100 + batch * 700
-    assert 4000 + own_ns / own <= max(ns) + 3000 + 2700
+    assert 4000 + own_ns / own <= max(ns) + 3000 + 2400
     # not known: every CTA does both
     assert loads(ops.shared_prefix_plan([0, batch], [0, prefix], 148))[1] == 148
 
