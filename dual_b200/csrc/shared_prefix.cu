@@ -15,7 +15,8 @@
 // and cuts them into one equal range per CTA (one CTA per SM), so a CTA works on one or a few segments, each a
 // part of one job, and a long prefix of a small batch still fills the GPU.  Own entries: the flattened token
 // axis is cut into one range per CTA as in tiered_decode_kernel.  Which CTAs do which part is the plan's: some the
-// prefixes and the others the own entries, or each both, the prefixes first.  shared_join_kernel joins the states; it is launched beside the first and waits for its end.
+// prefixes and the others the own entries, or each both, the prefixes first.  shared_join_kernel joins the states;
+// it is launched beside the first kernel and waits for its end.
 //
 // Prefix phase, warp-specialised; two streams of 128 rows x 128 entries alternate on the tensor core, one in
 // softmax while the other is in its products:
@@ -29,7 +30,7 @@
 // over its own S), a softmax warpgroup per stream turns S into P with one thread per row; the running maximum
 // moves only when it grows by more than 2^8.
 // Own phase: K rows (2 KiB, all kv heads) come by bulk copies, V rows by 16-byte copies; eight warps, one per kv head,
-// multiply 16 entries at a time with the 4 query heads of the group as the rows of warp-level products.
+// take 16 entries at a time, as the rows of warp-level products whose columns are the 4 query heads of the group.
 // All waits are bounded; one that runs out records DUAL_STATUS_WAIT_TIMEOUT and every role unwinds.
 #include <algorithm>
 #include <type_traits>
@@ -84,7 +85,8 @@ __device__ __forceinline__ void cp_async_16_zfill(void* dst, const void* src, bo
                : "memory");
 }
 __device__ __forceinline__ void cp_async_16_hint(void* dst, const void* src, uint64_t policy) {
-  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "l"(policy)
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src),
+               "l"(policy)
                : "memory");
 }
 __device__ __forceinline__ void cp_async_mbar_arrive_noinc(uint64_t* bar) {
@@ -107,11 +109,12 @@ struct Segment {
   __device__ __forceinline__ int tile(int s, int i) const { return single ? 2 * i + s : i; }  // the i-th of them
 };
 
-// Segment `i` of CTA `cta` (of `count`; the second is at `second` among the segments); false (and a status bit)
-// where it does not fit this call's tensors.
+// Segment `i` of this CTA (the second is at `second` among the segments behind the CTAs' records); false, and a
+// status bit, where it does not fit this call's tensors.
 __device__ __forceinline__ bool load_segment(const SharedPrefixParams& p, int second, int i, Segment& g) {
-  const int32_t* at = i == 0 ? p.plan + kPlanHeader + int64_t(blockIdx.x) * kCtaWords + 4
-                             : p.plan + kPlanHeader + int64_t(p.ctas) * kCtaWords + int64_t(second + i - 1) * kSegmentWords;
+  const int32_t* const records = p.plan + kPlanHeader;
+  const int32_t* at = i == 0 ? records + int64_t(blockIdx.x) * kCtaWords + 4
+                             : records + int64_t(p.ctas) * kCtaWords + int64_t(second + i - 1) * kSegmentWords;
   const int4 a = *reinterpret_cast<const int4*>(at), b = *(reinterpret_cast<const int4*>(at) + 1);
   g.tok0 = a.x;
   g.ntok = a.y;

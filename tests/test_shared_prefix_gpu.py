@@ -164,6 +164,8 @@ def test_plans_for_other_own_lengths(own):
     ([1, 1, 1, 1, 1], [1, 2, 3, 4, 5], [1, 1, 1, 1, 1]),
     ([6], [40], [3000, 0, 1, 0, 17, 900]),           # own entries that are split over CTAs
     ([300], [64], [1] * 300),                        # many requests per CTA
+    ([1, 200], [20000, 10], [3] * 201),              # one request with most of the states, more than the join's room
+    ([2], [9], [30000, 0]),                          # the same with own entries
 ])
 def test_empty_and_uneven_lists(sizes, prefixes, suffixes):
     c = Case(sizes, prefixes, suffixes, seed=len(suffixes))
