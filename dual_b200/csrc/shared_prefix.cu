@@ -1009,7 +1009,7 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_
     float top = M;
 #pragma unroll 4
     for (int e = 0; e < have; ++e) top = fmaxf(top, md[e * kState].x);
-    const float before = M == -INFINITY ? 0.f : exp2f(M - top);
+    const float before = M == -INFINITY ? 0.f : fast_exp2(M - top);
     M = top;
     D *= before;
     acc.x *= before;
@@ -1019,7 +1019,7 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_
 #pragma unroll 4
     for (int e = 0; e < have; ++e) {
       const float4 state = md[e * kState], v = in[e * kState + threadIdx.x];
-      const float w = state.x == -INFINITY ? 0.f : exp2f(state.x - M);
+      const float w = state.x == -INFINITY ? 0.f : fast_exp2(state.x - M);
       D += w * state.y;
       acc.x += w * v.x;
       acc.y += w * v.y;
