@@ -199,3 +199,16 @@ def test_no_tokens():
     empty = {k: a[k][:0] for k in ("locations", "positions", "q", "k", "v", "q_out")}
     ops.rope_set_kv_buffer(**{**a, **empty})
     assert torch.equal(a["k_local"], before["k_local"]) and torch.equal(a["v_local"], before["v_local"])
+
+
+def test_pools_with_a_page_axis_and_one_token_of_a_wide_buffer():
+    """Pools [slots, 1, 8, 128], and a single token whose tensors have strides of a larger buffer."""
+    a = inputs(3, 128, True, torch.int32, seed=12)
+    before = snapshot(a)
+    paged = {k: a[k].unsqueeze(1) for k in ("k_local", "v_local")}
+    one = {k: a[k][1:2] for k in ("locations", "positions", "q", "k", "v", "q_out")}
+    ops.rope_set_kv_buffer(**{**a, **paged, **one})
+    only = torch.tensor([False, True, False], device=DEV)
+    ref, size = check(a, before, False, 1e-6, only)
+    close(a["q_out"][1:2], (ref[1:2], size[1:2]), "q")
+    assert torch.equal(a["q_out"][0].view(torch.int16), before["q_out"][0].view(torch.int16))

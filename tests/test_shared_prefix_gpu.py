@@ -388,3 +388,33 @@ def test_on_a_side_stream_between_other_work():
     for out, lse in outs:
         assert torch.equal(out, outs[0][0]) and torch.equal(lse, outs[0][1])
     c.check(*outs[0])
+
+
+def test_two_calls_at_once():
+    """Two batches on two streams, each with a workspace of its own, beside each other."""
+    cases = [Case([40], [2000], mixed(40), seed=51), Case([10, 20], [900, 3000], mixed(30), banks=1, remote=0.2, seed=52)]
+    wrappers = [wrapper_for(c) for c in cases]
+    streams = [torch.cuda.Stream(DEV) for _ in cases]
+    for c, w in zip(cases, wrappers):
+        w.plan(c.gi, c.pi, c.prefix_pages, c.ii, c.own_pages, 32, 8, 128, 1)
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(15):
+        for i, (c, w, stream) in enumerate(zip(cases, wrappers, streams)):
+            with torch.cuda.stream(stream):
+                outs[i].append(w.run_return_lse(c.q, (c.k, c.v), *c.peers(), c.prefix_pages, c.own_pages, c.C, SCALE))
+    torch.cuda.synchronize()
+    for c, w, many in zip(cases, wrappers, outs):
+        assert w.status() == 0
+        for out, lse in many:
+            assert torch.equal(out, many[0][0]) and torch.equal(lse, many[0][1])
+        c.check(*many[0])
+
+
+def test_an_empty_batch():
+    w = wrapper_for(Case([1], [5], [1], seed=1))
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    w.plan([0], [0], none, torch.zeros(1, dtype=torch.int32), none, 32, 8, 128, 1)
+    pool = torch.zeros((4, 8, 128), dtype=torch.bfloat16, device=DEV)
+    out, lse = w.run_return_lse(torch.empty((0, 32, 128), dtype=torch.bfloat16, device=DEV), (pool, pool))
+    assert out.shape == (0, 32, 128) and lse.shape == (0, 32)
