@@ -20,7 +20,7 @@ constexpr int kRopeWarpRows = 8;                                               /
 constexpr int kRopeParts = (kNumQoHeads + 2 * kNumKvHeads) / kRopeWarpRows;   // warps per token: 6
 constexpr int kQParts = kNumQoHeads / kRopeWarpRows;                          // 4 of them hold q
 constexpr int kRopeThreads = kRopeParts * 32;
-constexpr int kRopeBlocks = 4;                                                // blocks per SM
+constexpr int kRopeBlocks = 4;  // blocks per SM: 32,768 tokens 142 us (3: 161, 5 with fewer registers: 174)
 static_assert(kNumKvHeads == kRopeWarpRows, "one warp holds a token's k rows, one its v rows");
 
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
