@@ -33,7 +33,6 @@
 // take 16 entries at a time, as the rows of warp-level products whose columns are the 4 query heads of the group.
 // All waits are bounded; one that runs out records DUAL_STATUS_WAIT_TIMEOUT and every role unwinds.
 #include <algorithm>
-#include <type_traits>
 #include <vector>
 
 #include "dual_b200.h"
@@ -413,8 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
       auto slot_free = [&](int slot) {
         if (leader) tc::commit(slot_empty + slot);
       };
-      bool residual = false;
-      // O_s (+)= P_s V, in the two parts in which the softmax hands P over (entries 32..127, 0..31)
+      // O_s (+)= P_s V, high parts and residuals, in the two parts in which the softmax hands P over (entries 32..127, 0..31)
       auto issue_pv = [&](int s, int slot, bool first) -> bool {
         const uint32_t np = s == 0 ? np0 : np1;
         const uint32_t v_base = base + slot_offset(slot);
@@ -430,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
             const uint32_t ph = tP + 32 * (kb >> 1) + 8 * (kb & 1);
             if (leader) {
               tc::mma_bf16_ts(tO, ph, vdesc, kIdescPV, (!first || part > 0 || k > 0) ? 1u : 0u);
-              if (residual) tc::mma_bf16_ts(tO, ph + 16, vdesc, kIdescPV, 1u);
+              tc::mma_bf16_ts(tO, ph + 16, vdesc, kIdescPV, 1u);
             }
           }
         }
@@ -467,7 +465,6 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
         if (!load_segment(p, second, i, g)) continue;
         const int ntiles = __reduce_max_sync(0xffffffffu, g.tiles());
         const bool single = __reduce_max_sync(0xffffffffu, int(g.single)) != 0;
-        residual = __reduce_max_sync(0xffffffffu, g.flags & kSegResidual) != 0;
         ok = wait_warp(q_full, uint32_t(nq) & 1u);
         ++nq;
         if (single) {
@@ -537,7 +534,6 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
         Segment g;
         if (!load_segment(p, second, i, g)) continue;
         const int n = g.tiles_of(s), len = g.kv1 - g.kv0;
-        const bool residual = (g.flags & kSegResidual) != 0;
         float m_used = -INFINITY, d_sum = 0.f;  // m_used in the scaled (log2) domain
         for (int j = 0; j < n; ++j) {
           if (!wait_warp(s_full + s, uint32_t(ns) & 1u)) {
@@ -595,35 +591,30 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
           }
           const uint64_t scale2 = f2_pack(scale, scale), neg_m2 = f2_pack(-m_used, -m_used);
           uint64_t rs2[4] = {0, 0, 0, 0};  // packed partial row sums, four independent chains
-          auto emit_p = [&](const float* xc, int col, auto lo_tag) {
-            constexpr bool kLo = decltype(lo_tag)::value;
+          // P enters P V as a bf16 pair, as in tiered_decode_kernel: rounded to bf16 alone a weight is off by up to
+          // 2^-8, which shows where the weights sit on a few entries, at any length.  The pair costs 3 to 6 % where
+          // the tensor core bounds (64 requests over 32,768 entries and up to 512 own: 55.5 -> 58.9 us; 66 -> 74 in a
+          // long loop under the power cap) and nothing where bytes do.  Words go out four at a time: eight at a time spilled registers (60.6 us).
+          auto emit = [&](const float* xc, int col) {
 #pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {  // 16 entries: 8 high words, 8 residual words
-              uint32_t hi[8], lo[8];
+            for (int sub = 0; sub < 4; ++sub) {  // 8 entries: 4 high words, 4 residual words
+              uint32_t hi[4], lo[4];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
+              for (int e = 0; e < 4; ++e) {
                 float t0, t1;
-                f2_unpack(f2_fma(f2_pack(xc[16 * sub + 2 * e], xc[16 * sub + 2 * e + 1]), scale2, neg_m2), t0, t1);
+                f2_unpack(f2_fma(f2_pack(xc[8 * sub + 2 * e], xc[8 * sub + 2 * e + 1]), scale2, neg_m2), t0, t1);
                 const float p0 = fast_exp2(t0), p1 = fast_exp2(t1);
                 const uint64_t pp = f2_pack(p0, p1);
                 rs2[e & 3] = f2_add(rs2[e & 3], pp);
                 hi[e] = pack_bf16x2(p0, p1);
-                if (kLo) {
-                  const uint64_t hh = f2_pack(__uint_as_float(hi[e] << 16), __uint_as_float(hi[e] & 0xffff0000u));
-                  float l0, l1;
-                  f2_unpack(f2_sub(pp, hh), l0, l1);
-                  lo[e] = pack_bf16x2(l0, l1);
-                }
+                const uint64_t hh = f2_pack(__uint_as_float(hi[e] << 16), __uint_as_float(hi[e] & 0xffff0000u));
+                float l0, l1;
+                f2_unpack(f2_sub(pp, hh), l0, l1);
+                lo[e] = pack_bf16x2(l0, l1);
               }
-              tc::st8u(tS + col + 8 * sub, hi);
-              if (kLo) tc::st8u(tS + col + 16 + 8 * sub, lo);
+              tc::st4u(tS + col + 4 * sub, hi);
+              tc::st4u(tS + col + 16 + 4 * sub, lo);
             }
-          };
-          auto emit = [&](const float* xc, int col) {
-            if (residual)
-              emit_p(xc, col, std::true_type{});
-            else
-              emit_p(xc, col, std::false_type{});
           };
           auto mask32 = [&](float* xc, int col) {
             if (needs_mask) {
@@ -1038,18 +1029,12 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_
 
 }  // namespace
 
-// P enters P V with its bf16 residual where a prefix has fewer than this many entries, as in the append
-// kernel: rounding P to bf16 costs up to 2^-9 of each term, and on short rows, where a few keys of opposite
-// sign can cancel, that shows in the output.
-namespace {
-constexpr int64_t kResidualMaxEntries = 1024;
-}
-
 int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_indptr, int groups, int ctas,
                            int64_t own_entries, int32_t* words, int64_t max_words) {
   // What a CTA takes, in ns, measured on a B200 with all CTAs at work: a prefix's first tile and last state; a
   // segment's; a kv tile with two query tiles, with one; own entries' first tile and last state; a tile of 16 of
-  // them; a request's state.
+  // them; a request's state.  (A kv tile with two query tiles at 2,550 or 2,700: 200 requests over 20,000 entries
+  // 104 -> 109, 112 us, 64 over 4,096 20.8 -> 23.4, 23.6, none better by more than 5 %.)
   constexpr int64_t kPrefixStart = 5000, kSegmentNs = 3000, kPairNs = 2400, kSingleNs = 1350, kOwnStart = 4000,
                     kOwnTile = 1100, kOwnRequest = 700;
   struct Block {
@@ -1160,7 +1145,7 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
     w[3] = b.kv0 + segs[i].first;
     w[4] = b.kv0 + segs[i].last;
     w[5] = int32_t(uint32_t(state));
-    w[6] = flags | (b.len < kResidualMaxEntries ? kSegResidual : 0);
+    w[6] = flags;
     state += int64_t(kState) * b.ntok;
   };
   int32_t* more = words + v.segment_at();

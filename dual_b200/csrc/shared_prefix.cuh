@@ -26,8 +26,7 @@ constexpr int kSegmentWords = 8;
 constexpr int kBlockRequests = 64;    // requests of a block: two query tiles of 32 requests x 4 heads
 constexpr int kStateGroups = kHeadDim / 4 + 1;
 constexpr int kState = kStateGroups * kGqa;  // 16-byte units
-constexpr int kSegResidual = 1;       // flags: P enters P V with its bf16 residual
-constexpr int kSegDeep = 2;           // no segment of this CTA has a second query tile: the ring has its room
+constexpr int kSegDeep = 2;           // flag: no segment of this CTA has a second query tile: the ring has its room
 
 struct PlanView {
   const int32_t* words;
