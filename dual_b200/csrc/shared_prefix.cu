@@ -33,6 +33,7 @@
 // take 16 entries at a time, as the rows of warp-level products whose columns are the 4 query heads of the group.
 // All waits are bounded; one that runs out records DUAL_STATUS_WAIT_TIMEOUT and every role unwinds.
 #include <algorithm>
+#include <cfloat>
 #include <vector>
 
 #include "dual_b200.h"
@@ -57,6 +58,9 @@ constexpr int kSoftmaxThreads = kSoftmaxWarps * 32;
 constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
 constexpr int kThreads = (kMmaWarp + 1) * 32;  // 416
 constexpr float kRescaleThreshold = 8.0f;      // log2 units: p stays <= 256 between rescales
+// The running maximum while no score was above -inf.  Finite: scores of -inf then get the weight 2^-inf = 0, where a
+// maximum of -inf would give 2^(-inf + inf); and lower than any other, so the first finite score replaces it.
+constexpr float kNoMax = -FLT_MAX;
 
 constexpr int kQBytes = kRows * 256;           // 32 KB: [128 rows x 128 dims] bf16
 constexpr int kSlotBytes = kBN * 256;          // 32 KB: [128 entries x 128 dims] bf16
@@ -534,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
         Segment g;
         if (!load_segment(p, second, i, g)) continue;
         const int n = g.tiles_of(s), len = g.kv1 - g.kv0;
-        float m_used = -INFINITY, d_sum = 0.f;  // m_used in the scaled (log2) domain
+        float m_used = kNoMax, d_sum = 0.f;  // m_used in the scaled (log2) domain
         for (int j = 0; j < n; ++j) {
           if (!wait_warp(s_full + s, uint32_t(ns) & 1u)) {
             ok = false;
@@ -791,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
       it.init(own_lo, own_hi, p.indptr, p.batch, lane);
       uint32_t qb[8][2];
       float o[8][4];  // dims 16 d + gi and + 8, columns 2 ci and 2 ci + 1
-      float m0 = -INFINITY, m1 = -INFINITY, d0 = 0.f, d1 = 0.f;  // of those columns
+      float m0 = kNoMax, m1 = kNoMax, d0 = 0.f, d1 = 0.f;  // of those columns
 #pragma unroll
       for (int d = 0; d < 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
       int cur_b = -1, n_seen = 0;
@@ -900,7 +904,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
           if (gi == 0)
             *reinterpret_cast<float2*>(dst + (kStateGroups - 1) * (kGqa * 4)) =
                 ci < 2 ? make_float2(m0, d0) : make_float2(m1, d1);
-          m0 = m1 = -INFINITY;
+          m0 = m1 = kNoMax;
           d0 = d1 = 0.f;
         }
       }
@@ -980,7 +984,7 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   const int n = n_pre + n_own;  // states 0 .. n_pre - 1 are the prefix's, the others the request's own
-  float M = -INFINITY, D = 0.f;
+  float M = kNoMax, D = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = 0, turn = 0; i0 < n; i0 += room, ++turn) {
     const int have = min(room, n - i0);
@@ -1000,7 +1004,7 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_
     float top = M;
 #pragma unroll 4
     for (int e = 0; e < have; ++e) top = fmaxf(top, md[e * kState].x);
-    const float before = M == -INFINITY ? 0.f : fast_exp2(M - top);
+    const float before = fast_exp2(M - top);
     M = top;
     D *= before;
     acc.x *= before;
@@ -1010,7 +1014,7 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_
 #pragma unroll 4
     for (int e = 0; e < have; ++e) {
       const float4 state = md[e * kState], v = in[e * kState + threadIdx.x];
-      const float w = state.x == -INFINITY ? 0.f : fast_exp2(state.x - M);
+      const float w = fast_exp2(state.x - M);
       D += w * state.y;
       acc.x += w * v.x;
       acc.y += w * v.y;
@@ -1019,12 +1023,12 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_
     }
     __syncthreads();  // before the next copies
   }
-  const float inv = n > 0 ? 1.f / D : 0.f;  // no entries at all: output 0, LSE -inf
+  const float inv = D == 0.f ? 0.f : 1.f / D;  // no entries, or no score above -inf: output 0, LSE -inf
   const int row = h * kGqa + r;
   __nv_bfloat16* orow = p.out + int64_t(b) * p.out_stride_tok + int64_t(row) * p.out_stride_head;
   *reinterpret_cast<uint2*>(orow + cg * 4) =
       make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-  if (p.lse != nullptr && cg == 0) p.lse[int64_t(b) * kNumQoHeads + row] = n > 0 ? M + log2f(D) : -INFINITY;
+  if (p.lse != nullptr && cg == 0) p.lse[int64_t(b) * kNumQoHeads + row] = M + log2f(D);
 }
 
 }  // namespace

@@ -129,8 +129,9 @@ int dual_decode_noalloc_status(uint32_t* value_out, int device, void* stream);
  * and share the prefix list prefix_indices[prefix_indptr[g] .. prefix_indptr[g+1)); request b besides
  * has its own list unified_indices[kv_indptr[b] .. kv_indptr[b+1)), as in dual_tiered_decode:
  *   out_b = softmax(sm_scale q_b [K_prefix; K_own]^T) [V_prefix; V_own],   lse base 2.
- * Any list may be empty; where both are, out = 0 and lse = -inf.  Equal to dual_tiered_decode over the
- * concatenated lists, but a prefix is read once per 64 requests, not once per request.
+ * Any list may be empty; where both are, or no score is above -inf, out = 0 and lse = -inf.  Equal to
+ * dual_tiered_decode over the concatenated lists (which gives NaN once 16 scores in a row are -inf), but a
+ * prefix is read once per 64 requests, not once per request.
  *
  * dual_shared_prefix_plan (host): from HOST copies of group_indptr and prefix_indptr ([groups + 1],
  * starting at 0; group_indptr[groups] is the batch), writes the work plan (int32 words) and returns its
