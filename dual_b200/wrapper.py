@@ -166,8 +166,13 @@ class SharedPrefixDecodeWrapper:
         self._buffers = dict(indptr=paged_kv_indptr_buffer, indices=paged_kv_indices_buffer,
                              prefix=prefix_indices_buffer, plan=plan_buffer)
         for name, t in self._buffers.items():
-            if use_cuda_graph and (t is None or t.dtype != torch.int32 or t.device != self.device):
-                raise ValueError(f"CUDA graphs need an int32 {name} buffer on {self.device}")
+            if t is None:
+                if use_cuda_graph:
+                    raise ValueError(f"CUDA graphs need an int32 {name} buffer on {self.device}")
+            elif t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.device != self.device:
+                raise ValueError(f"the {name} buffer must be contiguous int32 [n] on {self.device}")
+            elif name == "plan" and t.data_ptr() % 16:
+                raise ValueError("the plan buffer must be 16-byte aligned")
         self._batch = None
         self._sm_scale = None
 
