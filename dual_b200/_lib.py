@@ -52,6 +52,8 @@ SIGNATURES = {
     "dual_shared_prefix_plan": (C.c_int, [
         VP, VP, C.c_int, C.c_int, C.c_int64, VP, C.c_int64, C.POINTER(C.c_int64)]),
     "dual_shared_prefix_workspace_size": (C.c_int, [VP, C.c_int64, C.POINTER(C.c_size_t)]),
+    "dual_shared_prefix_limits": (C.c_int, [
+        C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t), C.POINTER(C.c_int64)]),
     "dual_shared_prefix_decode": (C.c_int, [
         VP, C.c_int64, C.c_int64,              # q, strides
         VP, VP, C.c_int64, C.c_int64,          # k_local, v_local, local stride, capacity

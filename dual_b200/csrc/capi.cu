@@ -198,6 +198,16 @@ int dual_shared_prefix_workspace_size(const int32_t* plan_host, int64_t plan_wor
   return DUAL_OK;
 }
 
+int dual_shared_prefix_limits(int batch, int groups, int num_ctas, size_t* workspace_bytes, int64_t* plan_words) {
+  g_last_error.clear();
+  if (batch < 0 || groups < 0 || num_ctas <= 0 || num_ctas > 65535 || !workspace_bytes || !plan_words)
+    return fail(DUAL_EINVAL, "bad shared-prefix limits arguments");
+  *workspace_bytes = 256 + dual::shared_prefix_own_bytes(batch, num_ctas) +
+                     size_t(dual::shared_prefix_most_states(batch, num_ctas)) * 16;
+  *plan_words = dual::shared_prefix_most_words(batch, groups, num_ctas);
+  return DUAL_OK;
+}
+
 int dual_shared_prefix_decode(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_local,
                               const void* v_local, int64_t local_stride_bytes, int64_t local_capacity,
                               const void* const* peer_k, const void* const* peer_v, int num_peers,

@@ -87,6 +87,21 @@ inline size_t shared_prefix_own_bytes(int batch, int ctas) {
   return size_t(ctas + batch) * kNumKvHeads * kState * 16;
 }
 
+// Partial prefix states (16-byte units) and words of the largest plan of a batch: the plan cuts jobs only where a CTA's
+// run ends, so there are at most ctas - 1 segments more than jobs, each with the states of up to 64 requests, and of the
+// segments that are not a CTA's first at most one per job.  A block needs a group that holds a request.
+inline int64_t shared_prefix_most_states(int batch, int ctas) {
+  return int64_t(kState) * (int64_t(batch) * kNumKvHeads + int64_t(ctas - 1) * (batch < kBlockRequests ? batch : kBlockRequests));
+}
+inline int64_t shared_prefix_most_words(int batch, int groups, int ctas) {
+  PlanView v{};
+  v.ctas = ctas;
+  v.requests = batch;
+  v.blocks = int((int64_t(batch) + int64_t(kBlockRequests - 1) * (groups < batch ? groups : batch)) / kBlockRequests);
+  v.segments = v.blocks * kNumKvHeads;
+  return v.total();
+}
+
 // Writes the plan (when `words` has room for it) and returns its size in words.  `own_entries`: how many entries of
 // their own the requests have in all, for the balance (negative: not known).
 int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_indptr, int groups, int ctas,

@@ -149,8 +149,18 @@ def shared_prefix_plan(group_indptr, prefix_indptr, num_ctas: int = 0, own_entri
     return plan
 
 
+def shared_prefix_limits(batch: int, groups: int, num_ctas: int = 0) -> Tuple[int, int]:
+    """(Workspace bytes, plan words) that are enough for every plan of up to ``batch`` requests in up to ``groups``
+    groups, whatever the lengths of the prefixes and of the own lists: what a serving program allocates once."""
+    nbytes, words = C.c_size_t(0), C.c_int64(0)
+    _lib.check(_lib.load().dual_shared_prefix_limits(int(batch), int(groups), int(num_ctas) or default_ctas(0),
+                                                     C.byref(nbytes), C.byref(words)))
+    return int(nbytes.value), int(words.value)
+
+
 def shared_prefix_workspace_size(plan: torch.Tensor) -> int:
-    """Workspace bytes of a call with this (host) plan."""
+    """Workspace bytes of a call with this (host) plan.  A plan for another number of own entries can need more:
+    ``shared_prefix_limits`` covers them all."""
     if plan.device.type != "cpu" or plan.dtype is not torch.int32 or not plan.is_contiguous():
         raise ValueError("plan must be a host plan of shared_prefix_plan")
     n = C.c_size_t(0)

@@ -144,7 +144,8 @@ class SharedPrefixDecodeWrapper:
     ``prefix_indices[prefix_indptr[g] .. prefix_indptr[g + 1]]`` and have entries of their own, ``indices`` by
     ``indptr``.  ``plan`` is called once per step (it builds the work plan of the prefixes on the host) and ``run``
     once per layer.  For CUDA graphs pass ``use_cuda_graph=True`` and the buffers that ``plan`` shall fill: the
-    captured ``run`` reads them again at every replay.
+    captured ``run`` reads them again at every replay.  ``ops.shared_prefix_limits(batch, groups)`` says how many bytes
+    of workspace and how many words of ``plan_buffer`` every step of such batches gets by with.
     """
 
     def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD", use_cuda_graph: bool = False,
@@ -206,7 +207,8 @@ class SharedPrefixDecodeWrapper:
             raise ValueError(f"CUDA graphs keep their batch: {self._batch}, got {batch}")
         need = ops.shared_prefix_workspace_size(words)
         if self._ws_bytes < need:
-            raise ValueError(f"float_workspace_buffer too small: need {need} bytes")
+            raise ValueError(f"float_workspace_buffer too small: need {need} bytes (any plan of such a batch: "
+                             f"{ops.shared_prefix_limits(batch, gi.numel() - 1, self._num_ctas)[0]})")
         self._plan = self._fill("plan", words, non_blocking)
         self._prefix = self._fill("prefix", prefix_indices, non_blocking)
         self._indptr = self._fill("indptr", indptr, non_blocking)

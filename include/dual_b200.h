@@ -130,8 +130,8 @@ int dual_decode_noalloc_status(uint32_t* value_out, int device, void* stream);
  * has its own list unified_indices[kv_indptr[b] .. kv_indptr[b+1)), as in dual_tiered_decode:
  *   out_b = softmax(sm_scale q_b [K_prefix; K_own]^T) [V_prefix; V_own],   lse base 2.
  * Any list may be empty; where both are, or no score is above -inf, out = 0 and lse = -inf.  Equal to
- * dual_tiered_decode over the concatenated lists (which gives NaN once 16 scores in a row are -inf), but a
- * prefix is read once per 64 requests, not once per request.
+ * dual_tiered_decode over the concatenated lists (there, scores of -inf can give NaN), but a prefix is read
+ * once per 64 requests, not once per request.
  *
  * dual_shared_prefix_plan (host): from HOST copies of group_indptr and prefix_indptr ([groups + 1],
  * starting at 0; group_indptr[groups] is the batch), writes the work plan (int32 words) and returns its
@@ -141,7 +141,10 @@ int dual_decode_noalloc_status(uint32_t* value_out, int device, void* stream);
  * nothing else, so a plan serves own lists of any length, best those of about that many entries.  num_ctas:
  * CTAs of the first launch (dual_decode_default_ctas).
  * dual_shared_prefix_workspace_size (host): bytes that a call with this plan needs; a larger workspace
- * serves smaller plans.  Its first 256 bytes hold the status word (clear it with dual_status_clear before
+ * serves smaller plans.  They move with own_entries, also where groups and prefixes stay.
+ * dual_shared_prefix_limits (host): workspace bytes and plan words that are enough for every plan of up to
+ * `batch` requests in up to `groups` groups, whatever the prefixes' lengths and own_entries.
+ * A workspace's first 256 bytes hold the status word (clear it with dual_status_clear before
  * the first call), the rest are partial states and may hold anything.
  * dual_shared_prefix_decode: two launches, the second (the join of the states) started as the first ends.  A plan that does not
  * fit the call (another batch, num_ctas or index list, a workspace too small for it) records
@@ -150,6 +153,7 @@ int dual_decode_noalloc_status(uint32_t* value_out, int device, void* stream);
 int dual_shared_prefix_plan(const int32_t* group_indptr_host, const int32_t* prefix_indptr_host, int groups,
                             int num_ctas, int64_t own_entries, int32_t* plan_host, int64_t max_words, int64_t* num_words);
 int dual_shared_prefix_workspace_size(const int32_t* plan_host, int64_t plan_words, size_t* bytes);
+int dual_shared_prefix_limits(int batch, int groups, int num_ctas, size_t* workspace_bytes, int64_t* plan_words);
 int dual_shared_prefix_decode(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k_local,
                               const void* v_local, int64_t local_stride_bytes, int64_t local_capacity,
                               const void* const* peer_k, const void* const* peer_v, int num_peers,
