@@ -200,9 +200,12 @@ class SharedPrefixDecodeWrapper:
         batch = int(gi[-1])
         if indptr.numel() != batch + 1:
             raise ValueError(f"indptr is for {indptr.numel() - 1} requests, the groups hold {batch}")
-        words = ops.shared_prefix_plan(gi, pi, self._num_ctas, int(indptr[-1]))
+        own_entries = int(indptr[-1])
+        words = ops.shared_prefix_plan(gi, pi, self._num_ctas, own_entries)
         if prefix_indices.numel() < int(pi[-1]):
             raise ValueError("prefix_indices is shorter than the prefixes")
+        if indices.numel() < own_entries:
+            raise ValueError("indices is shorter than the requests' own entries")
         if self._use_cuda_graph and self._batch not in (None, batch):
             raise ValueError(f"CUDA graphs keep their batch: {self._batch}, got {batch}")
         need = ops.shared_prefix_workspace_size(words)

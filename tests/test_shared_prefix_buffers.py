@@ -34,3 +34,38 @@ def test_plan_buffer_off_its_alignment(graph):
         SharedPrefixDecodeWrapper(torch.zeros(1 << 20, dtype=torch.uint8), use_cuda_graph=graph, num_ctas=8, **buffers)
     buffers["plan_buffer"] = buf()[4:]
     SharedPrefixDecodeWrapper(torch.zeros(1 << 20, dtype=torch.uint8), use_cuda_graph=graph, num_ctas=8, **buffers)
+
+
+def wrapper(graph, indptr=4, indices=64, prefix=64, plan=4096, fill=-9):
+    buf = lambda n: torch.full((n,), fill, dtype=torch.int32)  # noqa: E731
+    buffers = dict(paged_kv_indptr_buffer=buf(indptr), paged_kv_indices_buffer=buf(indices),
+                   prefix_indices_buffer=buf(prefix), plan_buffer=buf(plan))
+    w = SharedPrefixDecodeWrapper(torch.zeros(1 << 22, dtype=torch.uint8), use_cuda_graph=graph, num_ctas=8,
+                                  **(buffers if graph else {}))
+    return w, buffers
+
+
+def plan(w, prefix=20, listed=None, own=(5, 0, 7), own_listed=None):
+    """A plan of three requests of one group, up to the GPU call at its end; lists may be shorter than they should be."""
+    ids = lambda n: torch.arange(n, dtype=torch.int32)  # noqa: E731
+    ends = torch.tensor([0] + list(own)).cumsum(0)
+    try:
+        w.plan([0, 3], [0, prefix], ids(prefix if listed is None else listed), ends,
+               ids(sum(own) if own_listed is None else own_listed), 32, 8, 128, 1)
+    except ValueError as e:
+        if not str(e).startswith("expected a CUDA tensor"):
+            raise
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("own_listed", [0, 1, 11])
+def test_lists_shorter_than_their_indptr(graph, own_listed):
+    """With graphs the kernel is given the whole buffer, so it would read what an earlier plan left there."""
+    w, _ = wrapper(graph)
+    plan(w)
+    with pytest.raises(ValueError, match="indices is shorter than the requests' own entries"):
+        plan(w, own_listed=own_listed)
+    with pytest.raises(ValueError, match="prefix_indices is shorter"):
+        plan(w, listed=19)
+    plan(w, own_listed=12)
+    plan(w, own_listed=30)  # longer ones are taken
