@@ -182,8 +182,6 @@ class SharedPrefixDecodeWrapper:
         n = values.numel()
         buf = self._buffers[name]
         if buf is None or buf.numel() < n:
-            if self._use_cuda_graph:
-                raise ValueError(f"{n} words exceed the CUDA-graph {name} buffer")
             buf = self._buffers[name] = torch.empty(max(n, 1), dtype=torch.int32, device=self.device)
         buf[:n].copy_(values.to(torch.int32), non_blocking=non_blocking)
         return buf if self._use_cuda_graph else buf[:n]
@@ -198,6 +196,10 @@ class SharedPrefixDecodeWrapper:
             raise ValueError("dual_b200 decode is built for 32 q heads, 8 kv heads, head_dim 128, page_size 1")
         gi, pi = torch.as_tensor(group_indptr).to("cpu"), torch.as_tensor(prefix_indptr).to("cpu")
         batch = int(gi[-1])
+        lists = dict(indptr=indptr, prefix=prefix_indices, indices=indices)
+        for name, values in lists.items():
+            if values.dim() != 1 or values.is_floating_point():
+                raise ValueError(f"{name} must be a list of integers")
         if indptr.numel() != batch + 1:
             raise ValueError(f"indptr is for {indptr.numel() - 1} requests, the groups hold {batch}")
         own_entries = int(indptr[-1])
@@ -212,10 +214,13 @@ class SharedPrefixDecodeWrapper:
         if self._ws_bytes < need:
             raise ValueError(f"float_workspace_buffer too small: need {need} bytes (any plan of such a batch: "
                              f"{ops.shared_prefix_limits(batch, gi.numel() - 1, self._num_ctas)[0]})")
-        self._plan = self._fill("plan", words, non_blocking)
-        self._prefix = self._fill("prefix", prefix_indices, non_blocking)
-        self._indptr = self._fill("indptr", indptr, non_blocking)
-        self._indices = self._fill("indices", indices, non_blocking)
+        lists["plan"] = words
+        if self._use_cuda_graph:  # all of them before any is written: a captured run may be replayed after a refusal
+            for name, values in lists.items():
+                if self._buffers[name].numel() < values.numel():
+                    raise ValueError(f"{values.numel()} words exceed the CUDA-graph {name} buffer")
+        self._indptr, self._prefix, self._indices, self._plan = (
+            self._fill(name, values, non_blocking) for name, values in lists.items())
         ops.status_clear(self._float_workspace)  # the caller's buffer may hold anything
         self._plan_ptr, self._plan_words = self._plan.data_ptr(), self._plan.numel()
         self._indptr_ptr = self._indptr.data_ptr()

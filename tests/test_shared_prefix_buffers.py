@@ -69,3 +69,34 @@ def test_lists_shorter_than_their_indptr(graph, own_listed):
         plan(w, listed=19)
     plan(w, own_listed=12)
     plan(w, own_listed=30)  # longer ones are taken
+
+
+@pytest.mark.parametrize("short", [dict(indptr=3), dict(indices=11), dict(prefix=19), dict(plan=100)])
+def test_a_refused_plan_writes_nothing(short):
+    """A captured run is replayed on these buffers: a new work plan beside old lists would be a mixture of both."""
+    w, buffers = wrapper(True, **short)
+    with pytest.raises(ValueError, match="exceed the CUDA-graph"):
+        plan(w)
+    for name, t in buffers.items():
+        assert bool((t == -9).all()), name
+
+
+def test_a_plan_writes_each_buffer():
+    w, buffers = wrapper(True, indptr=4, indices=12, prefix=20)
+    plan(w)
+    assert buffers["paged_kv_indptr_buffer"].tolist() == [0, 5, 5, 12]
+    assert buffers["paged_kv_indices_buffer"].tolist() == list(range(12))
+    assert buffers["prefix_indices_buffer"].tolist() == list(range(20))
+
+
+@pytest.mark.parametrize("change", [
+    dict(prefix_indices=torch.zeros((1, 20), dtype=torch.int32)), dict(indices=torch.zeros((2, 6), dtype=torch.int32)),
+    dict(indptr=torch.tensor([[0, 5, 5, 12]])), dict(indices=torch.zeros(12)), dict(prefix_indices=torch.zeros(20))])
+def test_lists_of_another_shape_write_nothing(change):
+    w, buffers = wrapper(True)
+    lists = dict(prefix_indices=torch.zeros(20, dtype=torch.int32), indptr=torch.tensor([0, 5, 5, 12]),
+                 indices=torch.zeros(12, dtype=torch.int32))
+    with pytest.raises(ValueError, match="list of integers"):
+        w.plan([0, 3], [0, 20], **{**lists, **change}, num_qo_heads=32, num_kv_heads=8, head_dim=128, page_size=1)
+    for name, t in buffers.items():
+        assert bool((t == -9).all()), name
