@@ -181,6 +181,9 @@ int dual_shared_prefix_plan(const int32_t* group_indptr_host, const int32_t* pre
       return fail(DUAL_EINVAL, "group %d: negative length", g);
   if (groups > 0 && (group_indptr_host[0] != 0 || prefix_indptr_host[0] != 0))
     return fail(DUAL_EINVAL, "group_indptr and prefix_indptr start at 0");
+  if (groups > 0 && group_indptr_host[groups] > dual::kMaxRequests)
+    return fail(DUAL_EINVAL, "too many requests (%d)", group_indptr_host[groups]);
+  if (own_entries > INT32_MAX) return fail(DUAL_EINVAL, "own_entries must fit 32 bits, as kv_indptr does");
   try {
     *num_words = dual::shared_prefix_plan(group_indptr_host, prefix_indptr_host, groups, num_ctas, own_entries,
                                           plan_host, max_words);
@@ -200,7 +203,7 @@ int dual_shared_prefix_workspace_size(const int32_t* plan_host, int64_t plan_wor
 
 int dual_shared_prefix_limits(int batch, int groups, int num_ctas, size_t* workspace_bytes, int64_t* plan_words) {
   g_last_error.clear();
-  if (batch < 0 || groups < 0 || num_ctas <= 0 || num_ctas > 65535 || !workspace_bytes || !plan_words)
+  if (batch < 0 || batch > dual::kMaxRequests || groups < 0 || num_ctas <= 0 || num_ctas > 65535 || !workspace_bytes || !plan_words)
     return fail(DUAL_EINVAL, "bad shared-prefix limits arguments");
   *workspace_bytes = 256 + dual::shared_prefix_own_bytes(batch, num_ctas) +
                      size_t(dual::shared_prefix_most_states(batch, num_ctas)) * 16;
@@ -218,6 +221,7 @@ int dual_shared_prefix_decode(const void* q, int64_t q_stride_token, int64_t q_s
                               void* workspace, size_t workspace_bytes, int num_ctas, int device, void* stream) {
   g_last_error.clear();
   if (batch < 0) return fail(DUAL_EINVAL, "batch must be >= 0 (got %d)", batch);
+  if (batch > dual::kMaxRequests) return fail(DUAL_EINVAL, "batch must be at most %d", dual::kMaxRequests);
   if (batch == 0) return DUAL_OK;
   if (!q || !k_local || !v_local || !kv_indptr || !plan || !out || !workspace)
     return fail(DUAL_EINVAL, "null pointer argument");

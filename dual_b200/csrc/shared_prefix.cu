@@ -34,6 +34,7 @@
 // All waits are bounded; one that runs out records DUAL_STATUS_WAIT_TIMEOUT and every role unwinds.
 #include <algorithm>
 #include <cfloat>
+#include <stdexcept>
 #include <vector>
 
 #include "dual_b200.h"
@@ -1057,6 +1058,9 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
     }
   }
   const int32_t requests = groups > 0 ? group_indptr[groups] : 0;
+  int64_t all_states = 0;  // of the jobs, 16-byte units; cuts add to them below
+  for (const Block& b : blocks) all_states += int64_t(kState) * kNumKvHeads * b.ntok;
+  if (all_states > UINT32_MAX) throw std::length_error("more than 64 GiB of partial states");
   // Segments: the jobs' kv tiles laid end to end, cut into one run per CTA; a segment costs something beside its
   // tiles, so a CTA whose run crosses into another job gets less.  deal() fills CTAs up to a load and returns how
   // many it needs.
@@ -1135,6 +1139,8 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
   for (int c = 0; c < ctas; ++c) v.segments += std::max(0, cta[c + 1] - cta[c] - 1);
   v.requests = requests;
   v.blocks = int(blocks.size());
+  for (const Seg& seg : segs) v.state_size += int64_t(kState) * blocks[seg.block].ntok;
+  if (v.state_size > UINT32_MAX) throw std::length_error("more than 64 GiB of partial states");
   const int64_t size = v.total();
   if (words == nullptr || max_words < size) return size;
   std::fill(words, words + size, 0);

@@ -24,6 +24,7 @@ constexpr int kPlanHeader = 8;
 constexpr int kCtaWords = 12;
 constexpr int kSegmentWords = 8;
 constexpr int kBlockRequests = 64;    // requests of a block: two query tiles of 32 requests x 4 heads
+constexpr int kMaxRequests = 1 << 24;  // of a batch: their q and out are 275 GB
 constexpr int kStateGroups = kHeadDim / 4 + 1;
 constexpr int kState = kStateGroups * kGqa;  // 16-byte units
 constexpr int kSegDeep = 2;           // flag: no segment of this CTA has a second query tile: the ring has its room
@@ -104,6 +105,7 @@ inline int64_t shared_prefix_most_words(int batch, int groups, int ctas) {
 
 // Writes the plan (when `words` has room for it) and returns its size in words.  `own_entries`: how many entries of
 // their own the requests have in all, for the balance (negative: not known).
+// Throws where the states are more than the plan's 32-bit offsets can name (64 GiB).
 int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_indptr, int groups, int ctas,
                            int64_t own_entries, int32_t* words, int64_t max_words);
 cudaError_t launch_shared_prefix_decode(const SharedPrefixParams& p, cudaStream_t stream);

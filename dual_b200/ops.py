@@ -127,7 +127,10 @@ def _host_indptr(t, name: str) -> torch.Tensor:
     t = torch.as_tensor(t)
     if t.dim() != 1 or t.numel() < 1 or t.is_floating_point():
         raise ValueError(f"{name} must be a list of integers [groups + 1]")
-    return t.to("cpu", torch.int32).contiguous()
+    t = t.to("cpu")
+    if t.dtype is not torch.int32 and not torch.equal(t.to(torch.int32), t):
+        raise ValueError(f"{name} must fit 32 bits")
+    return t.to(torch.int32).contiguous()
 
 
 def shared_prefix_plan(group_indptr, prefix_indptr, num_ctas: int = 0, own_entries: int = -1) -> torch.Tensor:

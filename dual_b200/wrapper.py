@@ -194,7 +194,7 @@ class SharedPrefixDecodeWrapper:
         if (num_qo_heads, num_kv_heads, head_dim, page_size) != (ops.NUM_QO_HEADS, ops.NUM_KV_HEADS,
                                                                  ops.HEAD_DIM, 1):
             raise ValueError("dual_b200 decode is built for 32 q heads, 8 kv heads, head_dim 128, page_size 1")
-        gi, pi = torch.as_tensor(group_indptr).to("cpu"), torch.as_tensor(prefix_indptr).to("cpu")
+        gi, pi = ops._host_indptr(group_indptr, "group_indptr"), ops._host_indptr(prefix_indptr, "prefix_indptr")
         batch = int(gi[-1])
         lists = dict(indptr=indptr, prefix=prefix_indices, indices=indices)
         for name, values in lists.items():

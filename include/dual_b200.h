@@ -140,6 +140,7 @@ int dual_decode_noalloc_status(uint32_t* value_out, int device, void* stream);
  * of their own the requests have in all (negative if not known); it decides how many CTAs work on them and
  * nothing else, so a plan serves own lists of any length, best those of about that many entries.  num_ctas:
  * CTAs of the first launch (dual_decode_default_ctas).
+ * At most 2^24 requests and 64 GiB of partial states.
  * dual_shared_prefix_workspace_size (host): bytes that a call with this plan needs; a larger workspace
  * serves smaller plans.  They move with own_entries, also where groups and prefixes stay.
  * dual_shared_prefix_limits (host): workspace bytes and plan words that are enough for every plan of up to
