@@ -969,6 +969,7 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_
       }
     }
   }
+  if (own_last < own_first || own_first < 0 || (b == 0 && own_first != 0)) ok = false;  // no prefix sums from 0 on
   if (!ok && threadIdx.x == 0) atomicOr(p.status, kStatusBadLength);
   const int start = max(0, min(own_first, split.T)), end = max(start, min(own_last, split.T));
   constexpr int64_t kOwnStep = int64_t(kNumKvHeads) * kState;

@@ -147,8 +147,9 @@ int dual_decode_noalloc_status(uint32_t* value_out, int device, void* stream);
  * `batch` requests in up to `groups` groups, whatever the prefixes' lengths and own_entries.
  * A workspace's first 256 bytes hold the status word (clear it with dual_status_clear before
  * the first call), the rest are partial states and may hold anything.
- * dual_shared_prefix_decode: two launches, the second (the join of the states) started as the first ends.  A plan that does not
- * fit the call (another batch, num_ctas or index list, a workspace too small for it) records
+ * dual_shared_prefix_decode: two launches, the second (the join of the states) started as the first ends.
+ * A plan that does not fit the call (another batch, num_ctas or index list, a workspace too small for it) or
+ * a kv_indptr that is no list of prefix sums from 0 on (its end past num_indices too) records
  * DUAL_STATUS_BAD_LENGTH; the outputs are then not to be used.  Calls that share a workspace must not
  * overlap.  q, out: 16-byte aligned, element strides that are multiples of 8. */
 int dual_shared_prefix_plan(const int32_t* group_indptr_host, const int32_t* prefix_indptr_host, int groups,
