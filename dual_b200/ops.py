@@ -204,6 +204,8 @@ def _shared_prefix_launch(q, k_local, v_local, local_capacity, peer_k, peer_v, p
         raise ValueError("q must be bf16 [B, 32, 128] with contiguous head_dim")
     if out.dtype is not torch.bfloat16 or out.shape != shape or ot[2] != 1:
         raise ValueError("out must be bf16 [B, 32, 128] with contiguous head_dim")
+    if ot[1] < HEAD_DIM or (B > 1 and ot[0] < HEAD_DIM):
+        raise ValueError("out must not repeat rows")
     if (prefix_indices.dtype is not torch.int32 or prefix_indices.dim() != 1 or not prefix_indices.is_contiguous()
             or prefix_indices.get_device() != dev):
         raise ValueError("prefix_indices must be contiguous int32 [n] on q's device")

@@ -50,3 +50,20 @@ def test_empty_and_odd_indptrs_of_the_wrapper():
     for gi in ([], [[0, 2]], [0.0, 2.0]):
         with pytest.raises(ValueError, match="group_indptr must be a list of integers"):
             w.plan(gi, [0, 0], none, ends, none, 32, 8, 128, 1)
+
+
+@pytest.mark.parametrize("out", [torch.zeros((1, 32, 128), dtype=torch.bfloat16).expand(3, 32, 128),
+                                 torch.zeros((3, 1, 128), dtype=torch.bfloat16).expand(3, 32, 128),
+                                 torch.zeros(8192, dtype=torch.bfloat16).as_strided((3, 32, 128), (4096, 64, 1)),
+                                 torch.zeros(8192, dtype=torch.bfloat16).as_strided((3, 32, 128), (64, 128, 1))])
+def test_output_rows_that_share_memory(out):
+    from test_shared_prefix_plan import decode_args
+    with pytest.raises(ValueError, match="out must not repeat rows"):
+        ops.shared_prefix_decode(**{**decode_args(), "out": out})
+
+
+def test_one_request_has_no_token_stride():
+    from test_shared_prefix_plan import decode_args
+    out = torch.zeros((1, 32, 128), dtype=torch.bfloat16).as_strided((1, 32, 128), (0, 128, 1))
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        ops.shared_prefix_decode(**{**decode_args(B=1), "out": out})
