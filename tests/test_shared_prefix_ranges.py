@@ -54,8 +54,8 @@ def test_empty_and_odd_indptrs_of_the_wrapper():
 
 @pytest.mark.parametrize("out", [torch.zeros((1, 32, 128), dtype=torch.bfloat16).expand(3, 32, 128),
                                  torch.zeros((3, 1, 128), dtype=torch.bfloat16).expand(3, 32, 128),
-                                 torch.zeros(8192, dtype=torch.bfloat16).as_strided((3, 32, 128), (4096, 64, 1)),
-                                 torch.zeros(8192, dtype=torch.bfloat16).as_strided((3, 32, 128), (64, 128, 1))])
+                                 torch.zeros(16384, dtype=torch.bfloat16).as_strided((3, 32, 128), (4096, 64, 1)),
+                                 torch.zeros(16384, dtype=torch.bfloat16).as_strided((3, 32, 128), (64, 128, 1))])
 def test_output_rows_that_share_memory(out):
     from test_shared_prefix_plan import decode_args
     with pytest.raises(ValueError, match="out must not repeat rows"):
