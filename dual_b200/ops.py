@@ -9,6 +9,7 @@ inside CUDA-graph capture (no host synchronisation, no allocation) except
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -485,7 +486,11 @@ def merge_attention_states(states: Sequence[torch.Tensor], lses: Sequence[torch.
         sp, tok, head = s.data_ptr(), st[0] if T > 1 else row, st[1]
         if sp < oend and (sp, tok, head, e) != (op, ot, oh, oe) and _overlap(
                 op, oe * ot, osize, sp, e * tok, e * (head * (NUM_QO_HEADS - 1) + HEAD_DIM), T):
-            raise ValueError("out must be one of the states or not overlap them")
+            # of the same strides, their rows may still lie side by side: both start at multiples of one distance
+            step = math.gcd(oe * ot, oe * oh)
+            at = (sp - op) % step
+            if (e * tok, e * head) != (oe * ot, oe * oh) or at < oe * HEAD_DIM or at + e * HEAD_DIM > step:
+                raise ValueError("out must be one of the states or not overlap them")
         if not (l.dtype is torch.float32 and l.shape == lse_shape and l.is_contiguous() and l.get_device() == dev):
             raise ValueError(f"lses[{i}] must be contiguous fp32 [T, 32] on out's device")
         a = l.data_ptr()

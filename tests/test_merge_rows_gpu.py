@@ -58,3 +58,16 @@ def test_many_tokens_strided(T, n):
     ops.merge_attention_states(states, lses, buf[:, 1])
     close(buf[:, 1], None, want)
     assert torch.equal(buf[:, ::2], kept[:, ::2]) and torch.equal(wide, kept_wide)
+
+
+@pytest.mark.parametrize("T,n", [(40, 2), (2369, 2), (1185, 3)])
+def test_side_by_side_within_a_head(T, n):
+    """States and output in one buffer [T, 32, n + 1, 128]."""
+    g = torch.Generator(device=DEV).manual_seed(T)
+    buf = torch.empty((T, 32, n + 1, 128), dtype=BF, device=DEV).normal_(generator=g)
+    states, out = list(buf.unbind(2)[:n]), buf[:, :, n]
+    lses = [torch.empty((T, 32), device=DEV).normal_(generator=g) for _ in states]
+    want, kept = merged64(states, lses), buf.clone()
+    ops.merge_attention_states(states, lses, out)
+    close(out, None, want)
+    assert torch.equal(buf[:, :, :n], kept[:, :, :n])
