@@ -1000,6 +1000,7 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_
     }
     if (!mbar_wait_bounded(full, turn & 1)) {
       atomicOr(p.status, kStatusWaitTimeout);
+      mbar_wait_bounded(full, turn & 1);  // the block's shared memory must not go while copies still land in it
       break;
     }
     const float4* const md = in + (kStateGroups - 1) * kGqa + r;
