@@ -7,9 +7,11 @@
 // O / d, the base-2 log-sum-exp m + log2 d.  All states are held in 32 bits.
 // Read by each request alone, a prefix of P entries costs a batch of B requests 4096 B P bytes; here the
 // group's requests are the rows of one matrix product, and every K / V row is read once per block of 64
-// requests.  Up to about 64 requests the bytes bound it (64 requests x 16,384 operations per entry of 4,096
-// bytes are 256 operations per byte, the ratio of the card's measured rates is 251), above that the
-// tensor cores and the exponentials; the requests' own entries are bound by bytes.
+// requests.  Up to 32 requests the bytes bound it.  From 33 on a block is two query tiles, and a kv tile then takes
+// 2.5 us for its 64 KB (3.8 TB/s over the card): the chain softmax -> P V -> Q K -> softmax of the two streams sets
+// the pace, tensor core and exponentials each at about half their rate.  (By the card's measured rates bytes would
+// bound up to 64 requests: 256 operations per byte against 251.)  The requests' own entries are bound by the rate at
+// which an SM takes them, 16 in 1.1 us.
 //
 // Work.  Prefixes: a job is (block of up to 64 requests, kv head); the plan lays the jobs' kv tiles end to end
 // and cuts them into one equal range per CTA (one CTA per SM), so a CTA works on one or a few segments, each a
@@ -599,7 +601,8 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
           // P enters P V as a bf16 pair, as in tiered_decode_kernel: rounded to bf16 alone a weight is off by up to
           // 2^-8, which shows where the weights sit on a few entries, at any length.  The pair costs 3 to 6 % where
           // the tensor core bounds (64 requests over 32,768 entries and up to 512 own: 55.5 -> 58.9 us; 66 -> 74 in a
-          // long loop under the power cap) and nothing where bytes do.  Words go out four at a time: eight at a time spilled registers (60.6 us).
+          // long loop under the power cap) and nothing where bytes do.  Words go out four at a time: eight at a time
+          // spilled registers (60.6 us).
           auto emit = [&](const float* xc, int col) {
 #pragma unroll
             for (int sub = 0; sub < 4; ++sub) {  // 8 entries: 4 high words, 4 residual words
@@ -939,7 +942,7 @@ constexpr int kMaxJoinStates = 24;
 // every state is one bulk copy into shared memory, up to `room` of them in flight at once, and the code is short.
 // (Read by the threads themselves, 64 bytes per four lanes, 18 states took 9 us.)  Thread = (row, column group).
 __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_constant__ SharedPrefixParams p, int room) {
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   float4* const in = reinterpret_cast<float4*>(smem);  // [room][kState]
   uint64_t* const full = reinterpret_cast<uint64_t*>(smem + room * (kState * 16));
   const int b = blockIdx.x / kNumKvHeads, h = blockIdx.x % kNumKvHeads;
@@ -1119,7 +1122,7 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
   };
   // Either every CTA does its part of the prefixes and then of the own entries, or some do the one and the others
   // the other, each part's latencies then being paid by its own CTAs only: 16 requests over 32,768 entries and up
-  // to 256 own took 45.3 us the first way and 38.7 the second, 64 over 32,768 and up to 512 took 65.4 and 54.7.
+  // to 256 own take 43.5 us the first way and 36.7 the second, 64 over 32,768 and up to 512 65.3 and 59.4.
   int own_ctas = ctas;
   if (jobs > 0) {
     int64_t load = smallest([&](int64_t m) { return deal(m, false) <= ctas; });
@@ -1164,7 +1167,7 @@ int64_t shared_prefix_plan(const int32_t* group_indptr, const int32_t* prefix_in
   for (int c = 0; c < ctas; ++c) {
     // The last CTAs get the first runs, the first ones the own entries.  Consecutive CTAs share a pair of SMs, and
     // CTAs of the two kinds in one pair slow each other (with every other CTA of each kind, 256 requests over
-    // 16,384 entries and up to 600 own took 167 us instead of 120).
+    // 16,384 entries and up to 600 own took 167 us where they took 120 this way, before weights were bf16 pairs).
     int32_t* w = words + kPlanHeader + int64_t(ctas - 1 - c) * kCtaWords;
     w[0] = cta[c + 1] - cta[c];
     w[1] = int32_t((more - (words + v.segment_at())) / kSegmentWords);
