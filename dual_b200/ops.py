@@ -411,7 +411,7 @@ def rope_set_kv_buffer(k_local: torch.Tensor, v_local: torch.Tensor, locations: 
     layer's pools.  ``positions`` [n] name rows of ``cos_sin`` (fp32 [positions, rotary dims]: cosines, then
     sines); the first ``rotary dims`` of each head are turned, in pairs (j, j + half) or, ``interleaved``,
     (2j, 2j + 1).  With norm weights [128] bf16 each q / k head row is RMS-normalised first.  Token strides
-    are free (views of a fused qkv buffer).  Tokens with a bad position are skipped, rows with a bad slot are
+    are free (views of a fused qkv buffer); otherwise q, k, v, ``q_out`` and the pools do not overlap.  Tokens with a bad position are skipped, rows with a bad slot are
     not stored; both are recorded in ``status``."""
     ls = _pool_stride(k_local, "k_local")
     if not (v_local.shape == k_local.shape and v_local.dtype is k_local.dtype
